@@ -380,6 +380,42 @@ int h3k_attention_segments(const void* q, const void* k, const void* v, int64_t 
 int h3k_vae_heads(void* qkv, int32_t rows, int32_t heads, int32_t T, const float* rope, float eps, void* stream);
 int h3k_layer_norm(const float* x, int32_t rows, int32_t d, const float* w, const float* b, float eps, void* out, void* stream);
 
+/* ------------------------------------------------------------------------------------ microscaled 4-bit floating point
+ * Rows of e2m1 values (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) whose blocks share a scale, the 4-bit counterpart
+ * of the int8 rows above (no counterpart in the reference). A matrix [rows][K], K a multiple of 32, is
+ *   codes      two values a byte, the first in the low half; K / 2 bytes a row, rows contiguous
+ *   scales     a byte a block, in tiles of 128 rows x 4 blocks (512 bytes; the tiles of 128 rows one after another along K):
+ *              byte (row % 32) * 16 + (row / 32 % 4) * 4 + block % 4 of a tile. The tiles are whole: the bytes of rows and
+ *              blocks past the matrix are part of the buffer and must be 0 (the quantiser writes them)
+ *   row_scale  fp32 [rows], H3K_FP4_NV only
+ * H3K_FP4_MX: blocks of 32, scale 2^e as byte e + 127 (255: NaN). H3K_FP4_NV: blocks of 16, e4m3 scales.
+ * All pointers are device memory of the current device, 16-byte aligned (row_scale 4); work is queued on `stream`, and
+ * the calls may be captured into a graph. 0 rows: nothing is done. */
+#define H3K_FP4_MX 0
+#define H3K_FP4_NV 1
+#define H3K_BF16 0 /* element types */
+#define H3K_F16 1
+#define H3K_F32 2
+/* Bytes of the codes and scales of [rows][K] (either may be NULL). Host only. */
+int h3k_fp4_sizes(int32_t rows, int32_t K, int32_t format, uint64_t* code_bytes, uint64_t* scale_bytes);
+/* Quantises rows of K values of `type`, ldx elements apart (rows 16-byte aligned).
+ * MX: a block's scale is 2^e, e = max(floor(log2 max|x|) - 2, -127). NV: the row's scale g = 2^max(floor(log2 max|row|) -
+ * 10, -126), a block's scale c = e4m3(max|x| / (6 g)). The codes are x over the scales (0 where the block's scale is 0),
+ * rounded to the nearest value, ties to the even code, at most 6 in magnitude. An infinity or a NaN makes its block's
+ * scale (MX) or its row's (NV) a NaN, with codes of 0. row_scale: NULL for MX. */
+int h3k_quant_rows_fp4(const void* x, int32_t type, int64_t ldx, int32_t rows, int32_t K, int32_t format, void* codes, void* scales,
+                       float* row_scale, void* stream);
+/* The values that the codes stand for, code x block scale x row scale, rounded once to `type`; out's rows ldo apart.
+ * row_scale NULL: 1. */
+int h3k_dequant_rows_fp4(const void* codes, const void* scales, const float* row_scale, int32_t rows, int32_t K, int32_t format, int32_t type,
+                         void* out, int64_t ldo, void* stream);
+/* D[M][N] = A[M][K] B[N][K]^T of two such matrices of one format, fp32 accumulation, with h3k_gemm's epilogues (0 to 4) and
+ * arguments: a_scale [M] and b_scale [N] are the row scales (either may be NULL: 1); lda, ldb, a_chunks and a_rows_stride
+ * stay 0 (or K, K, 1, 0). N is a multiple of 8 (SwiGLU: 256, B's rows in 128-row [gate; value] groups; q/k/v: 3 inner).
+ * bias and b_scale are 16-byte aligned. The gated residual reads and writes x, whose rows must not alias another operand. */
+int h3k_gemm_fp4(const void* A, const void* A_scales, const void* B, const void* B_scales, int32_t format, const h3k_gemm_args* args,
+                 int32_t epilogue, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,338 @@
+// Quantisation of rows to microscaled 4-bit floating point and back (layouts in fp4.cuh).
+//
+// Both are bound by HBM: the quantiser reads a row once and keeps it in registers while the row's maximum is found (nv
+// has a scale a row), the inverse reads half a byte and writes two or four for each value. A thread takes runs of 16
+// values: an nv block, or half of an mx block whose two threads exchange their maxima by a shuffle.
+#include "common.hpp"
+#include "fp4.cuh"
+#include "ptx.cuh"
+
+#include <cuda_fp16.h>
+
+namespace h3 {
+
+namespace {
+
+// Sixteen consecutive values of a row, as loaded.
+template <Elem T>
+struct Run {
+    static constexpr int WORDS = T == Elem::f32 ? 16 : 8;
+    uint32_t w[WORDS];
+
+    __device__ __forceinline__ void load(const void* row, int c)
+    {
+        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(row) + size_t(c) * (T == Elem::f32 ? 4 : 2));
+#pragma unroll
+        for (int i = 0; i < WORDS / 4; ++i) {
+            const uint4 v = __ldg(p + i);
+            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+        }
+    }
+    // The bits of the largest magnitude as fp32 (an infinity or a NaN is larger than every number, a NaN than an
+    // infinity: magnitudes are compared as integers, which keeps both).
+    __device__ __forceinline__ uint32_t largest() const
+    {
+        uint32_t m = 0;
+        if constexpr (T == Elem::f32) {
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i)
+                m = max(m, w[i] & 0x7fffffffu);
+            return m;
+        } else {
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i)
+                m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+            m = max(m & 0xffffu, m >> 16);
+            return T == Elem::bf16 ? m << 16 : __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
+        }
+    }
+    __device__ __forceinline__ float2 pair(int i) const
+    {
+        if constexpr (T == Elem::f32) {
+            return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+        } else if constexpr (T == Elem::bf16) {
+            return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+        } else {
+            return __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        }
+    }
+};
+
+// Four pairs as e2m1 codes, the first value in the lowest bits; half to even, 6 at most.
+__device__ __forceinline__ uint32_t e2m1x8(float2 a, float2 b, float2 c, float2 d)
+{
+    uint32_t r;
+    asm("{\n\t.reg .b8 x, y, z, t;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 x, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 y, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 z, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %8, %7;\n\t"
+        "mov.b32 %0, {x, y, z, t};\n\t}"
+        : "=r"(r)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y), "f"(d.x), "f"(d.y));
+    return r;
+}
+
+// x >= 0 as e4m3 (half to even, 448 at most), and back.
+__device__ __forceinline__ uint32_t to_e4m3(float x)
+{
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(x));
+    return r & 0xffu;
+}
+__device__ __forceinline__ float from_e4m3(uint32_t b)
+{
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(b)));
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(h & 0xffffu)));
+}
+
+__device__ __forceinline__ float power_of_two(int e) // -127 <= e <= 127 (2^-127 is subnormal)
+{
+    return __uint_as_float(e > -127 ? uint32_t(e + 127) << 23 : 0x00400000u);
+}
+
+// The scale byte of a block whose largest magnitude has the bits `most`, and the sixteen codes of this thread's run.
+// rg: 1 / the row's scale (nv). A block (mx) or row (nv) with an infinity or a NaN has codes 0; its scale says NaN.
+template <Elem T, Fp4 F>
+__device__ __forceinline__ uint2 encode(const Run<T>& x, uint32_t most, float rg, uint32_t& byte)
+{
+    float2 q[8];
+    if constexpr (F == Fp4::mx) {
+        if (most >= 0x7f800000u) {
+            byte = 255;
+            return make_uint2(0, 0);
+        }
+        // 2^e with e = floor(log2 most) - 2: the division by it is exact, so the codes are those of the exact quotient
+        const int e = max(int(most >> 23) - 127 - 2, -127);
+        byte = uint32_t(e + 127);
+        const float inv = power_of_two(-e);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float2 v = x.pair(i);
+            q[i] = make_float2(v.x * inv, v.y * inv);
+        }
+    } else {
+        byte = to_e4m3(__fdiv_rn(__uint_as_float(most) * rg, 6.f));
+        const float c = from_e4m3(byte);
+        const float inv = c > 0.f ? __frcp_rn(c) : 0.f;
+        // x / c rounded to nearest from the reciprocal (one residual step: exact where c has four bits), so that a quotient
+        // on the border of two codes is seen as one
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float2 v = x.pair(i);
+            const float sx = v.x * rg, sy = v.y * rg;
+            const float qx = sx * inv, qy = sy * inv;
+            q[i] = make_float2(fmaf(fmaf(-qx, c, sx), inv, qx), fmaf(fmaf(-qy, c, sy), inv, qy));
+        }
+    }
+    return make_uint2(e2m1x8(q[0], q[1], q[2], q[3]), e2m1x8(q[4], q[5], q[6], q[7]));
+}
+
+__device__ __forceinline__ size_t scale_at(int row, int block, int tiles)
+{
+    return (size_t(row >> 7) * tiles + (block >> 2)) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
+}
+
+constexpr int QUANT_THREADS = 256;
+constexpr int QUANT_RUNS = 4; // runs of 16 values that a thread keeps
+
+// WARPS warps a row, QUANT_THREADS / 32 / WARPS rows a CTA. A row of more than WARPS x 32 x RUNS runs (only with eight
+// warps) is read twice instead of kept.
+template <Elem T, Fp4 F, int WARPS, int RUNS>
+__global__ void __launch_bounds__(QUANT_THREADS) quant_fp4_kernel(const void* x, int64_t ldx, int rows, int K, uint8_t* codes, uint8_t* scales,
+                                                                  float* row_scale)
+{
+    constexpr int ROWS = QUANT_THREADS / 32 / WARPS, STEP = WARPS * 32;
+    __shared__ uint32_t red[QUANT_THREADS / 32];
+    const int r = blockIdx.x * ROWS + warp_id() / WARPS;
+    const int t = threadIdx.x % STEP;
+    const int runs = K / 16, tiles = fp4_scale_tiles(K, F);
+    const bool in = r < rows;
+    const uint8_t* row = static_cast<const uint8_t*>(x) + (in ? size_t(r) * ldx * (T == Elem::f32 ? 4 : 2) : 0);
+
+    Run<T> keep[RUNS];
+    uint32_t most[RUNS];
+    uint32_t all = 0;
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i) {
+        most[i] = 0;
+        if (in && t + i * STEP < runs)
+            keep[i].load(row, (t + i * STEP) * 16);
+    }
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i)
+        if (in && t + i * STEP < runs) {
+            most[i] = keep[i].largest();
+            all = max(all, most[i]);
+        }
+    float rg = 1.f;
+    if constexpr (F == Fp4::nv) {
+        if (in)
+            for (int c = t + RUNS * STEP; c < runs; c += STEP) {
+                Run<T> a;
+                a.load(row, c * 16);
+                all = max(all, a.largest());
+            }
+        all = __reduce_max_sync(0xffffffffu, all);
+        if constexpr (WARPS > 1) {
+            if (lane_id() == 0)
+                red[warp_id()] = all;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < WARPS; ++i)
+                all = max(all, red[warp_id() / WARPS * WARPS + i]);
+        }
+        // 2^(floor(log2 max) - 10): block scales up to 2^11 / 6 = 341.3, under e4m3's 448
+        const int e = max(int(all >> 23) - 127 - 10, -126);
+        const bool number = all < 0x7f800000u;
+        rg = number ? power_of_two(-e) : 0.f; // 0 x infinity is a NaN, whose code is replaced below
+        if (in && t == 0)
+            row_scale[r] = number ? power_of_two(e) : __uint_as_float(0x7fffffffu);
+    }
+    const bool number = F == Fp4::mx || all < 0x7f800000u;
+    // The runs come in whole tiles of four scale bytes (2 runs a byte for mx); the tail's bytes and the rows past the
+    // tensor's are 0.
+    const int padded = tiles * 4 * fp4_block(F) / 16;
+    auto finish = [&](int c, const Run<T>& a, uint32_t m) {
+        uint32_t byte = 0;
+        uint2 code = make_uint2(0, 0);
+        const bool have = in && c < runs;
+        if constexpr (F == Fp4::mx)
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 1)); // the block's other half (both in the row: K is a multiple of 32)
+        if (have && number)
+            code = encode<T, F>(a, m, rg, byte);
+        if (have)
+            *reinterpret_cast<uint2*>(codes + size_t(r) * (K / 2) + size_t(c) * 8) = code;
+        // four lanes' (eight for mx) bytes into one word
+        constexpr int PER = fp4_block(F) / 16;
+        uint32_t word = byte << (8 * ((c / PER) & 3));
+#pragma unroll
+        for (int o = PER; o < 4 * PER; o <<= 1)
+            word |= __shfl_xor_sync(0xffffffffu, word, o);
+        if (c < padded && (c & (4 * PER - 1)) == 0 && (r >> 7) < (rows + 127) >> 7)
+            *reinterpret_cast<uint32_t*>(scales + scale_at(r, c / PER, tiles)) = word;
+    };
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i)
+        if (i * STEP < padded) // the same for the whole CTA: the shuffles see full warps
+            finish(t + i * STEP, keep[i], most[i]);
+    for (int c0 = RUNS * STEP; c0 < padded; c0 += STEP) {
+        const int c = c0 + t;
+        Run<T> a;
+        uint32_t m = 0;
+        if (in && c < runs) {
+            a.load(row, c * 16);
+            m = a.largest();
+        }
+        finish(c, a, m);
+    }
+}
+
+// A thread an output run of 16 values.
+template <Elem T, Fp4 F>
+__global__ void __launch_bounds__(256) dequant_fp4_kernel(const uint8_t* codes, const uint8_t* scales, const float* row_scale, int rows, int K,
+                                                          void* out, int64_t ldo)
+{
+    const int runs = K / 16, tiles = fp4_scale_tiles(K, F);
+    const size_t id = size_t(blockIdx.x) * 256 + threadIdx.x;
+    if (id >= size_t(rows) * runs)
+        return;
+    const int r = int(id / runs), c = int(id % runs);
+    const uint2 code = __ldg(reinterpret_cast<const uint2*>(codes + size_t(r) * (K / 2)) + c);
+    const uint32_t byte = __ldg(scales + scale_at(r, F == Fp4::mx ? c / 2 : c, tiles));
+    float scale;
+    if constexpr (F == Fp4::mx)
+        scale = byte == 255 ? __uint_as_float(0x7fffffffu) : power_of_two(int(byte) - 127);
+    else
+        scale = from_e4m3(byte);
+    const float g = row_scale ? __ldg(row_scale + r) : 1.f;
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        uint32_t h;
+        const uint16_t b = uint16_t(((i < 4 ? code.x : code.y) >> (8 * (i & 3))) & 0xffu);
+        asm("{\n\t.reg .b8 lo, hi;\n\tmov.b16 {lo, hi}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, lo;\n\t}" : "=r"(h) : "h"(b));
+        const float2 f = __half22float2(*reinterpret_cast<__half2*>(&h));
+        // code x block scale is exact (2 and 4 bits), so the product with the row's scale is the one rounding in fp32
+        v[2 * i] = f.x * scale * g, v[2 * i + 1] = f.y * scale * g;
+    }
+    if constexpr (T == Elem::f32) {
+        float4* d = reinterpret_cast<float4*>(static_cast<float*>(out) + size_t(r) * ldo + size_t(c) * 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            d[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    } else {
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (T == Elem::bf16) {
+                w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+            } else {
+                const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+        }
+        uint4* d = reinterpret_cast<uint4*>(static_cast<uint8_t*>(out) + (size_t(r) * ldo + size_t(c) * 16) * 2);
+        d[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        d[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+}
+
+template <Elem T, Fp4 F>
+void quant(const void* x, int64_t ldx, int rows, int K, void* codes, void* scales, float* row_scale, cudaStream_t s)
+{
+    const int runs = K / 16, all_rows = (rows + 127) / 128 * 128;
+    auto launch = [&](auto kernel, int warps) {
+        const int per = QUANT_THREADS / 32 / warps;
+        kernel<<<(all_rows + per - 1) / per, QUANT_THREADS, 0, s>>>(x, ldx, rows, K, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales),
+                                                                    row_scale);
+        H3_CUDA(cudaGetLastError());
+    };
+    // the fewest warps a row that keep it in QUANT_RUNS runs a thread
+    if (runs <= 32 * QUANT_RUNS)
+        launch(quant_fp4_kernel<T, F, 1, QUANT_RUNS>, 1);
+    else if (runs <= 64 * QUANT_RUNS)
+        launch(quant_fp4_kernel<T, F, 2, QUANT_RUNS>, 2);
+    else if (runs <= 128 * QUANT_RUNS)
+        launch(quant_fp4_kernel<T, F, 4, QUANT_RUNS>, 4);
+    else
+        launch(quant_fp4_kernel<T, F, 8, QUANT_RUNS>, 8);
+}
+
+template <Elem T, Fp4 F>
+void dequant(const void* codes, const void* scales, const float* row_scale, int rows, int K, void* out, int64_t ldo, cudaStream_t s)
+{
+    const size_t n = size_t(rows) * (K / 16);
+    dequant_fp4_kernel<T, F><<<unsigned((n + 255) / 256), 256, 0, s>>>(static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales),
+                                                                       row_scale, rows, K, out, ldo);
+    H3_CUDA(cudaGetLastError());
+}
+
+} // namespace
+
+void quant_rows_fp4(const void* x, Elem type, int64_t ldx, int rows, int K, Fp4 f, void* codes, void* scales, float* row_scale,
+                    cudaStream_t s)
+{
+    if (rows <= 0)
+        return;
+    const bool nv = f == Fp4::nv;
+    switch (type) {
+    case Elem::bf16: return (nv ? quant<Elem::bf16, Fp4::nv> : quant<Elem::bf16, Fp4::mx>)(x, ldx, rows, K, codes, scales, row_scale, s);
+    case Elem::f16: return (nv ? quant<Elem::f16, Fp4::nv> : quant<Elem::f16, Fp4::mx>)(x, ldx, rows, K, codes, scales, row_scale, s);
+    case Elem::f32: return (nv ? quant<Elem::f32, Fp4::nv> : quant<Elem::f32, Fp4::mx>)(x, ldx, rows, K, codes, scales, row_scale, s);
+    }
+}
+
+void dequant_rows_fp4(const void* codes, const void* scales, const float* row_scale, int rows, int K, Fp4 f, Elem type, void* out,
+                      int64_t ldo, cudaStream_t s)
+{
+    if (rows <= 0)
+        return;
+    const bool nv = f == Fp4::nv;
+    switch (type) {
+    case Elem::bf16: return (nv ? dequant<Elem::bf16, Fp4::nv> : dequant<Elem::bf16, Fp4::mx>)(codes, scales, row_scale, rows, K, out, ldo, s);
+    case Elem::f16: return (nv ? dequant<Elem::f16, Fp4::nv> : dequant<Elem::f16, Fp4::mx>)(codes, scales, row_scale, rows, K, out, ldo, s);
+    case Elem::f32: return (nv ? dequant<Elem::f32, Fp4::nv> : dequant<Elem::f32, Fp4::mx>)(codes, scales, row_scale, rows, K, out, ldo, s);
+    }
+}
+
+} // namespace h3

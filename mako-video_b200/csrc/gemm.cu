@@ -14,6 +14,7 @@
 //   swiglu      swiglu_rows: silu(gate) * value of fc1's [gate; value] halves
 #include "common.hpp"
 #include "gemm.cuh"
+#include "gemm_epi.cuh"
 #include "ptx.cuh"
 
 #include <algorithm>
@@ -25,7 +26,6 @@ namespace {
 constexpr int BM = 128;
 constexpr int KBYTES = 128;       // bytes of K per stage and row: 64 bf16 or 128 int8
 constexpr int STAGES = 4;
-constexpr int GROUP_M = 16;
 constexpr int NUM_THREADS = 192;  // 6 warps
 
 template <int BN, Epi EPI>
@@ -37,54 +37,6 @@ struct Smem {
     static constexpr int STAGING = (EPI == Epi::qkv || EPI == Epi::swiglu) ? BM * 256 : 0;
     static constexpr int TOTAL = STAGES * STAGE_BYTES + STAGING + 1024 /* alignment slack */ + 256 /* barriers */;
 };
-
-// Destination tensor maps of the TMA-store epilogues. q/k/v: one per rank that owns heads, (dim, q/k/v x head slot,
-// row) over that rank's block of this rank's rows, in its receive buffer (fused exchange) or in this rank's send
-// layout. SwiGLU: m[0] is the output [M][ldo] (box 64 columns x 128 rows).
-struct OutMaps {
-    CUtensorMap m[8];
-};
-
-__device__ __forceinline__ void epi_bar() { asm volatile("bar.sync 1, 128;" ::: "memory"); } // the 4 epilogue warps
-
-__device__ __forceinline__ void tma_store_3d(const void* tmap, const void* smem_src, int32_t c0, int32_t c1, int32_t c2)
-{
-    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
-                     reinterpret_cast<uint64_t>(tmap)),
-                 "r"(smem_u32(smem_src)), "r"(c0), "r"(c1), "r"(c2)
-                 : "memory");
-}
-__device__ __forceinline__ void tma_store_2d(const void* tmap, const void* smem_src, int32_t c0, int32_t c1)
-{
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(reinterpret_cast<uint64_t>(tmap)),
-                 "r"(smem_u32(smem_src)), "r"(c0), "r"(c1)
-                 : "memory");
-}
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_read0() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait0() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-
-__device__ __forceinline__ void tile_coords(int tile, int tiles_m, int tiles_n, int& tm, int& tn)
-{
-    const int group_size = GROUP_M * tiles_n;
-    const int g = tile / group_size;
-    const int first_m = g * GROUP_M;
-    const int gm = min(tiles_m - first_m, GROUP_M);
-    const int in_group = tile - g * group_size;
-    tm = first_m + in_group % gm;
-    tn = in_group / gm;
-}
-
-__device__ __forceinline__ float silu(float g) { return g / (1.0f + __expf(-g)); }
-
-__device__ __forceinline__ void store_bf16x32(__nv_bfloat16* dst, const float* v)
-{
-    uint4* d = reinterpret_cast<uint4*>(dst);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        d[i] = make_uint4(pack_bf16x2(v[8 * i + 0], v[8 * i + 1]), pack_bf16x2(v[8 * i + 2], v[8 * i + 3]),
-                          pack_bf16x2(v[8 * i + 4], v[8 * i + 5]), pack_bf16x2(v[8 * i + 6], v[8 * i + 7]));
-}
 
 // Loads `NCHUNK` 32-column chunks of this thread's accumulator row (starting at column `col0`) as floats, dequantising
 // int32 with the row and column scales when IS_I8.
@@ -424,26 +376,7 @@ void launch(const void* A, const void* B, const GemmParams& p, cudaStream_t s)
     smem_opt_in(gemm_kernel<BN, EPI, IS_I8>, smem, opt_in);
     const int tiles = ((p.M + BM - 1) / BM) * (p.N / BN);
     const int grid = std::min(tiles, num_sms());
-    OutMaps om{};
-    if constexpr (EPI == Epi::qkv) {
-        // rank r's block of this rank's rows: in r's receive buffer (fused exchange) or in this rank's send layout
-        const int P = p.inner / 128 / p.heads_per_rank;
-        const uint64_t slots = 3 * uint64_t(p.heads_per_rank);
-        const uint64_t odims[3] = {128, slots, uint64_t(p.rows_local)};
-        const uint64_t ostr[2] = {256, slots * 256};
-        const uint32_t obox[3] = {64, 1, 128};
-        for (int r = 0; r < P; ++r) {
-            const size_t block = size_t(p.peer_out[r] ? p.my_rank : r) * p.rows_local * slots * 128;
-            const __nv_bfloat16* base = static_cast<const __nv_bfloat16*>(p.peer_out[r] ? p.peer_out[r] : p.out) + block;
-            om.m[r] = make_tmap(CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, odims, ostr, obox);
-        }
-    }
-    if constexpr (EPI == Epi::swiglu) {
-        const uint64_t odims[2] = {uint64_t(p.N / 2), uint64_t(p.M)};
-        const uint64_t ostr[1] = {uint64_t(p.ldo) * 2};
-        const uint32_t obox[2] = {64, 128};
-        om.m[0] = make_tmap(CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.out, odims, ostr, obox);
-    }
+    const OutMaps om = out_maps<EPI>(p, p.rows_local);
     gemm_kernel<BN, EPI, IS_I8><<<grid, NUM_THREADS, smem, s>>>(ta, tb, p, om);
     H3_CUDA(cudaGetLastError());
 }

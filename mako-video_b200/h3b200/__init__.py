@@ -15,6 +15,8 @@ LIB_PATH = os.path.join(PKG, "lib", "libh3b200.so")
 
 H3_OK, H3_ERR_ARG, H3_ERR_CUDA, H3_ERR_STATE, H3_ERR_DEVICE = 0, 1, 2, 3, 4
 EPI_BF16, EPI_F32, EPI_QKV, EPI_GATE_RESID, EPI_SWIGLU, EPI_S32 = range(6)
+FP4_MX, FP4_NV = 0, 1
+BF16, F16, F32 = 0, 1, 2
 INT8_QKV, INT8_OUT, INT8_FC1, INT8_FC2 = 1, 2, 4, 8
 
 # Model shapes (h3_config): the benchmark's synthetic stacks and the real MiniMax-H3.
@@ -164,6 +166,10 @@ SIGNATURES = {
     "h3vae_destroy": (None, [_P]),
     "h3k_attention_segments": (ctypes.c_int, [_P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32, _P, _I64, _P]),
     "h3k_vae_heads": (ctypes.c_int, [_P, _I32, _I32, _I32, _P, _F, _P]),
+    "h3k_fp4_sizes": (ctypes.c_int, [_I32, _I32, _I32, _P, _P]),
+    "h3k_quant_rows_fp4": (ctypes.c_int, [_P, _I32, _I64, _I32, _I32, _I32, _P, _P, _P, _P]),
+    "h3k_dequant_rows_fp4": (ctypes.c_int, [_P, _P, _P, _I32, _I32, _I32, _I32, _P, _I64, _P]),
+    "h3k_gemm_fp4": (ctypes.c_int, [_P, _P, _P, _P, _I32, ctypes.POINTER(h3k_gemm_args), _I32, _P]),
     "h3k_layer_norm": (ctypes.c_int, [_P, _I32, _I32, _P, _P, _F, _P, _P]),
 }
 
@@ -294,6 +300,13 @@ def packed_order(dense_rows, frames, ph, pw):
     src = np.zeros(frames * ph * pw, np.int32)
     check(lib().h3k_video_order(ctypes.byref(g), src.ctypes.data))
     return np.concatenate([np.arange(dense_rows, dtype=np.int64), dense_rows + src.astype(np.int64)])
+
+
+def fp4_sizes(rows, K, format):
+    """h3k_fp4_sizes: bytes of the codes and of the block scales of a 4-bit matrix [rows][K] (host only)."""
+    codes, scales = ctypes.c_uint64(), ctypes.c_uint64()
+    check(lib().h3k_fp4_sizes(rows, K, format, ctypes.byref(codes), ctypes.byref(scales)))
+    return codes.value, scales.value
 
 
 def nccl_unique_id():
