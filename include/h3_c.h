@@ -416,6 +416,33 @@ int h3k_dequant_rows_fp4(const void* codes, const void* scales, const float* row
 int h3k_gemm_fp4(const void* A, const void* A_scales, const void* B, const void* B_scales, int32_t format, const h3k_gemm_args* args,
                  int32_t epilogue, void* stream);
 
+/* ------------------------------------------------------------------------------------------- packed documents
+ * Attention over documents of different lengths packed in one set of rows (clips, prompts or requests of one batch), each
+ * seeing its own keys and those of a prefix that all of them share: the masked form of h3k_attention_segments (no
+ * counterpart in the reference). Query row i of document d sees the key rows [0, prefix) and [k_start[d], k_start[d + 1])
+ * (a key in both counts once): out_i = softmax(scale q_i . k_j) v_j over them, zeros where it sees none or no score is
+ * above -infinity. Rows of out in no document stay as they are, and what lies in keys that a row does not see (a NaN,
+ * say) does not reach it. With self-attention q_start and k_start are the same array, and the prefix's rows a document.
+ * Softmax statistics and sums are fp32; the probabilities are rounded to the values' type for their product with v.
+ * Heads h of q and out use kv head h / (heads / kv_heads). */
+typedef struct h3k_packed_args {
+    const void* q; /* (row, head, dim) at q + row * q_stride + head * head_dim + dim, and so on; 16-byte aligned rows */
+    const void* k;
+    const void* v;
+    void* out;
+    int64_t q_stride, k_stride, v_stride, out_stride; /* elements between rows */
+    int32_t type;                                     /* H3K_BF16 or H3K_F16 */
+    int32_t heads, kv_heads, head_dim;                /* heads a multiple (1 to 64) of kv_heads; head_dim 64 or 128 */
+    int32_t q_rows, k_rows;                           /* rows of q and out, of k and v */
+    int32_t docs, prefix;
+    const int32_t* q_start; /* [docs + 1], ascending, in device memory, read when the work runs (a replayed graph sees */
+    const int32_t* k_start; /* new values): starts out of order or out of the rows are a device error (h3k_check), after */
+                            /* which what the call wrote is not to be used; nothing outside the rows is touched */
+    float scale;            /* 0: 1 / sqrt(head_dim) */
+} h3k_packed_args;
+/* Queued on `stream`, no scratch and no synchronisation; may be captured into a graph. */
+int h3k_attention_packed(const h3k_packed_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

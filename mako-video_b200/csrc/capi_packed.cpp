@@ -1,10 +1,13 @@
-// The C ABI's 4-bit floating point calls (h3k_fp4_sizes, h3k_quant_rows_fp4, h3k_dequant_rows_fp4, h3k_gemm_fp4): checks
-// of the arguments, then the launchers of fp4.cuh.
+// The C ABI's 4-bit floating point calls (h3k_fp4_sizes, h3k_quant_rows_fp4, h3k_dequant_rows_fp4, h3k_gemm_fp4) and the
+// attention over packed documents (h3k_attention_packed): checks of the arguments, then the launchers of fp4.cuh and
+// attention_packed.cuh.
 #include "h3_c.h"
 
+#include "attention_packed.cuh"
 #include "common.hpp"
 #include "fp4.cuh"
 
+#include <cmath>
 #include <functional>
 #include <initializer_list>
 #include <stdexcept>
@@ -157,6 +160,38 @@ int h3k_gemm_fp4(const void* A, const void* A_scales, const void* B, const void*
         p.qn_w = a->qn_w, p.kn_w = a->kn_w, p.eps = a->eps, p.inner = a->inner, p.heads_per_rank = a->heads_per_rank;
         p.rows_local = a->rows_local, p.a_scale = a->a_scale, p.b_scale = a->b_scale;
         h3::gemm_fp4(A, A_scales, B, B_scales, f, p, h3::Epi(epilogue), static_cast<cudaStream_t>(stream));
+    });
+}
+
+int h3k_attention_packed(const h3k_packed_args* a, void* stream)
+{
+    return h3::run_guarded([&] {
+        const char* call = "h3k_attention_packed";
+        need(a, call, "null argument");
+        need(a->type == H3K_BF16 || a->type == H3K_F16, call, "the values are bf16 or f16");
+        need(a->head_dim == 64 || a->head_dim == 128, call, "heads have 64 or 128 dims");
+        need(a->heads > 0 && a->kv_heads > 0 && a->heads % a->kv_heads == 0 && a->heads / a->kv_heads <= 64 && a->kv_heads <= 65535, call,
+             "heads must be a multiple (at most 64) of kv_heads");
+        need(a->q_rows >= 0 && a->k_rows >= 0 && a->docs >= 0, call, "a negative number of rows or documents");
+        need(a->prefix >= 0 && a->prefix <= a->k_rows, call, "the prefix must lie in the key rows");
+        need(a->scale >= 0.f && std::isfinite(a->scale), call, "the scale must be positive (0: 1 / sqrt(head_dim))");
+        if (a->q_rows == 0 || a->docs == 0)
+            return;
+        need(a->q && a->out && a->q_start && a->k_start && (a->k_rows == 0 || (a->k && a->v)), call, "null argument");
+        need(aligned(a->q, 16) && aligned(a->k, 16) && aligned(a->v, 16) && aligned(a->out, 16) && aligned(a->q_start, 4) && aligned(a->k_start, 4),
+             call, "a pointer is not aligned");
+        const int64_t q_width = int64_t(a->heads) * a->head_dim, k_width = int64_t(a->kv_heads) * a->head_dim;
+        auto rows_ok = [](int rows, int64_t stride, int64_t width) { return rows <= 1 || (stride >= width && stride % 8 == 0); };
+        need(rows_ok(a->q_rows, a->q_stride, q_width) && rows_ok(a->q_rows, a->out_stride, q_width) && rows_ok(a->k_rows, a->k_stride, k_width) &&
+                 rows_ok(a->k_rows, a->v_stride, k_width),
+             call, "rows must not overlap and be 16 bytes aligned");
+        device_only(call, {a->q, a->k, a->v, a->out, a->q_start, a->k_start});
+        h3::PackedAttnParams p;
+        p.q = a->q, p.k = a->k, p.v = a->v, p.out = a->out, p.q_stride = a->q_stride, p.k_stride = a->k_stride, p.v_stride = a->v_stride;
+        p.out_stride = a->out_stride, p.f16 = a->type == H3K_F16, p.heads = a->heads, p.kv_heads = a->kv_heads, p.head_dim = a->head_dim;
+        p.q_rows = a->q_rows, p.k_rows = a->k_rows, p.docs = a->docs, p.prefix = a->prefix, p.q_start = a->q_start, p.k_start = a->k_start;
+        p.scale = a->scale > 0.f ? a->scale : 1.f / std::sqrt(float(a->head_dim));
+        h3::attention_packed(p, static_cast<cudaStream_t>(stream));
     });
 }
 

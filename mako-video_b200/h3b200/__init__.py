@@ -84,6 +84,14 @@ class h3k_gemm_args(ctypes.Structure):
                 ("a_scale", ctypes.c_void_p), ("b_scale", ctypes.c_void_p)]
 
 
+class h3k_packed_args(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("out", ctypes.c_void_p),
+                ("q_stride", ctypes.c_int64), ("k_stride", ctypes.c_int64), ("v_stride", ctypes.c_int64), ("out_stride", ctypes.c_int64),
+                ("type", ctypes.c_int32), ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("q_rows", ctypes.c_int32), ("k_rows", ctypes.c_int32), ("docs", ctypes.c_int32), ("prefix", ctypes.c_int32),
+                ("q_start", ctypes.c_void_p), ("k_start", ctypes.c_void_p), ("scale", ctypes.c_float)]
+
+
 class h3k_cube_grid(ctypes.Structure):
     _fields_ = [("dense_rows", ctypes.c_int32), ("frames", ctypes.c_int32), ("ph", ctypes.c_int32), ("pw", ctypes.c_int32)]
 
@@ -170,6 +178,7 @@ SIGNATURES = {
     "h3k_quant_rows_fp4": (ctypes.c_int, [_P, _I32, _I64, _I32, _I32, _I32, _P, _P, _P, _P]),
     "h3k_dequant_rows_fp4": (ctypes.c_int, [_P, _P, _P, _I32, _I32, _I32, _I32, _P, _I64, _P]),
     "h3k_gemm_fp4": (ctypes.c_int, [_P, _P, _P, _P, _I32, ctypes.POINTER(h3k_gemm_args), _I32, _P]),
+    "h3k_attention_packed": (ctypes.c_int, [ctypes.POINTER(h3k_packed_args), _P]),
     "h3k_layer_norm": (ctypes.c_int, [_P, _I32, _I32, _P, _P, _F, _P, _P]),
 }
 
