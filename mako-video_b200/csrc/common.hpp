@@ -47,6 +47,31 @@ void smem_opt_in(Kernel* kernel, int bytes, std::atomic<uint64_t>& done)
     done.fetch_or(bit, std::memory_order_release);
 }
 
+// How many clusters of `size` CTAs of a kernel the current device holds at once (one object per kernel; asked once per
+// device and size). `c` describes the launch: block and shared memory, with the cluster dimension as its first attribute.
+struct ClusterLimits {
+    std::atomic<int> found[64][9] = {}; // + 1
+    template <class Kernel>
+    int at_once(Kernel* kernel, cudaLaunchConfig_t c, int size)
+    {
+        int dev = 0;
+        cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
+        if (dev < 0 || dev > 63 || size < 1 || size > 8)
+            return 0;
+        int n = found[dev][size].load(std::memory_order_relaxed) - 1;
+        if (n < 0) {
+            cudaLaunchAttribute at = c.attrs[0];
+            at.val.clusterDim.x = unsigned(size);
+            c.attrs = &at;
+            c.numAttrs = 1;
+            c.gridDim = dim3(unsigned(size));
+            cuda_check(cudaOccupancyMaxActiveClusters(&n, kernel, &c), "cudaOccupancyMaxActiveClusters");
+            found[dev][size].store(n + 1, std::memory_order_relaxed);
+        }
+        return n;
+    }
+};
+
 // True when a kernel may dereference p: device or managed memory, or pinned host memory mapped into the device's
 // address space (null counts as accessible; callers check their own required arguments).
 bool device_accessible(const void* p);

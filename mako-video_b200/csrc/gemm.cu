@@ -14,7 +14,7 @@
 //   swiglu      swiglu_rows: silu(gate) * value of fc1's [gate; value] halves
 #include "common.hpp"
 #include "gemm.cuh"
-#include "gemm_epi.cuh"
+#include "gemm_tiles.cuh"
 #include "ptx.cuh"
 
 #include <algorithm>
@@ -37,6 +37,26 @@ struct Smem {
     static constexpr int STAGING = (EPI == Epi::qkv || EPI == Epi::swiglu) ? BM * 256 : 0;
     static constexpr int TOTAL = STAGES * STAGE_BYTES + STAGING + 1024 /* alignment slack */ + 256 /* barriers */;
 };
+
+// Destination tensor maps of the TMA-store epilogues. q/k/v: one per rank that owns heads, (dim, q/k/v x head slot,
+// row) over that rank's block of this rank's rows, in its receive buffer (fused exchange) or in this rank's send
+// layout. SwiGLU: m[0] is the output [M][ldo] (box 64 columns x 128 rows).
+struct OutMaps {
+    CUtensorMap m[8];
+};
+
+__device__ __forceinline__ void epi_bar() { asm volatile("bar.sync 1, 128;" ::: "memory"); } // the 4 epilogue warps
+
+__device__ __forceinline__ float silu(float g) { return g / (1.0f + __expf(-g)); }
+
+__device__ __forceinline__ void store_bf16x32(__nv_bfloat16* dst, const float* v)
+{
+    uint4* d = reinterpret_cast<uint4*>(dst);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        d[i] = make_uint4(pack_bf16x2(v[8 * i + 0], v[8 * i + 1]), pack_bf16x2(v[8 * i + 2], v[8 * i + 3]),
+                          pack_bf16x2(v[8 * i + 4], v[8 * i + 5]), pack_bf16x2(v[8 * i + 6], v[8 * i + 7]));
+}
 
 // Loads `NCHUNK` 32-column chunks of this thread's accumulator row (starting at column `col0`) as floats, dequantising
 // int32 with the row and column scales when IS_I8.
@@ -376,7 +396,26 @@ void launch(const void* A, const void* B, const GemmParams& p, cudaStream_t s)
     smem_opt_in(gemm_kernel<BN, EPI, IS_I8>, smem, opt_in);
     const int tiles = ((p.M + BM - 1) / BM) * (p.N / BN);
     const int grid = std::min(tiles, num_sms());
-    const OutMaps om = out_maps<EPI>(p, p.rows_local);
+    OutMaps om{};
+    if constexpr (EPI == Epi::qkv) {
+        // rank r's block of this rank's rows: in r's receive buffer (fused exchange) or in this rank's send layout
+        const int P = p.inner / 128 / p.heads_per_rank;
+        const uint64_t slots = 3 * uint64_t(p.heads_per_rank);
+        const uint64_t odims[3] = {128, slots, uint64_t(p.rows_local)};
+        const uint64_t ostr[2] = {256, slots * 256};
+        const uint32_t obox[3] = {64, 1, 128};
+        for (int r = 0; r < P; ++r) {
+            const size_t block = size_t(p.peer_out[r] ? p.my_rank : r) * p.rows_local * slots * 128;
+            const __nv_bfloat16* base = static_cast<const __nv_bfloat16*>(p.peer_out[r] ? p.peer_out[r] : p.out) + block;
+            om.m[r] = make_tmap(CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, odims, ostr, obox);
+        }
+    }
+    if constexpr (EPI == Epi::swiglu) {
+        const uint64_t odims[2] = {uint64_t(p.N / 2), uint64_t(p.M)};
+        const uint64_t ostr[1] = {uint64_t(p.ldo) * 2};
+        const uint32_t obox[2] = {64, 128};
+        om.m[0] = make_tmap(CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.out, odims, ostr, obox);
+    }
     gemm_kernel<BN, EPI, IS_I8><<<grid, NUM_THREADS, smem, s>>>(ta, tb, p, om);
     H3_CUDA(cudaGetLastError());
 }

@@ -1,20 +1,26 @@
 // The projection GEMM on microscaled 4-bit rows (layouts in fp4.cuh): tcgen05.mma kind::mxf4 / kind::mxf4nvf4 with the
 // block scales in TMEM, fp32 accumulation, the row scales and the step's epilogues on the way out.
 //
-// One persistent kernel, one CTA per SM, the roles of the bf16 GEMM: warp 0 loads (TMA tiles of 128 bytes = 256 values of
-// K, 128-byte swizzled; the scale tiles by plain bulk copies), warp 1 issues, warps 2..5 are the epilogue. Per stage the
-// issuing thread copies the stage's scale tiles from shared memory into TMEM (tcgen05.cp, in order before the MMAs that
-// read them) and runs four M = 128, N = 256, K = 64 MMAs.
+// One CTA per SM: warp 0 loads (TMA tiles of 128 bytes = 256 values of K, 128-byte swizzled; the scale tiles by plain bulk
+// copies), warp 1 issues, warps 2..9 are the epilogue. Per stage the issuer copies the stage's scale tiles from shared
+// memory into TMEM (tcgen05.cp, in order before the MMAs that read them) and runs four M = 128, N = 256, K = 64 MMAs. The
+// issue itself is what a stage's 12 copies and 4 MMAs in 512 clocks strain: descriptors are made once a stage and the
+// warp stays converged (one lane chosen by elect.sync), which took 33024 x 15360 x 5120 without an epilogue from 1.68 ms
+// to 0.93.
 //
 // TMEM: two accumulators of 256 columns and the scales do not fit 512 columns side by side, and N = 256 is what keeps the
 // shared-memory reads of an MMA (12 KB) under its time, so the accumulators overlap in 96 columns:
 //   [0, 256) accumulator 0, [160, 416) accumulator 1, [416, 512) two buffers of one stage's scales (48 columns each)
-// An epilogue reads the shared columns first (into registers) and hands them on; the next tile's MMAs wait for that,
-// not for the whole epilogue. A scale buffer is written again only after the MMAs that read it are known to be complete
-// (the stage's `empty` barrier), two stages later: the stage between keeps the tensor core busy meanwhile.
+// The epilogue's eight warps take a finished accumulator into registers at once (128 columns a thread) and hand TMEM on;
+// the next tile's MMAs wait for that, not for the arithmetic and the stores. A scale buffer is written again only after
+// the MMAs that read it are known to be complete (the stage's `empty` barrier), two stages later: the stage between keeps
+// the tensor core busy meanwhile.
+//
+// With fewer tiles than SMs (few rows), the K of a tile is split over the CTAs of a cluster instead of one CTA walking
+// tiles; they leave their sums in shared memory and each finishes a share of the tile from all of them, in their order.
 #include "common.hpp"
 #include "fp4.cuh"
-#include "gemm_epi.cuh"
+#include "gemm_tiles.cuh"
 #include "ptx.cuh"
 
 #include <algorithm>
@@ -27,27 +33,33 @@ namespace {
 constexpr int BM = 128, BN = 256;
 constexpr int KSTAGE = 256;          // values of K per stage: 128 bytes of codes a row
 constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128;
-constexpr int NUM_THREADS = 192;
-constexpr int ACC1 = 160, OVERLAP = 96; // accumulator 1's first column, the columns that it shares with accumulator 0
+constexpr int EPI_WARPS = 8;
+constexpr int NUM_THREADS = 64 + 32 * EPI_WARPS;
+constexpr int STAGES = 3;
+constexpr int ACC1 = 160;            // accumulator 1's first column
 constexpr int SCALE_COL = 416, SCALE_BUF = 48;
+constexpr int MAX_SPLIT = 8;         // CTAs of a cluster
 
-constexpr bool staged(Epi e) { return e == Epi::qkv || e == Epi::swiglu; } // output tiles through shared memory and TMA stores
-
-template <Epi EPI, Fp4 F>
+template <Fp4 F>
 struct Fp4Smem {
     // scale tiles of a stage: 4 (nv) or 2 (mx) along K for A's 128 rows and twice as many for B's 256
     static constexpr int KT = KSTAGE / (4 * fp4_block(F));
     static constexpr int SF_BYTES = 3 * KT * 512;
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SF_BYTES;
-    static constexpr int STAGING = staged(EPI) ? BM * 256 : 0;
-    static constexpr int STAGES = staged(EPI) ? 3 : 4;
-    static constexpr int TOTAL = STAGES * STAGE_BYTES + STAGING + 1024 + 256;
+    static constexpr int OFF_STAGING = STAGES * STAGE_BYTES;             // 4 KB an epilogue warp: 32 rows of 128 bytes
+    static constexpr int OFF_COLS = OFF_STAGING + EPI_WARPS * 4096;      // its columns' scales and biases, 2 x 128 floats
+    static constexpr int OFF_BAR = OFF_COLS + EPI_WARPS * 1024;
+    static constexpr int TOTAL = OFF_BAR + 256 + 1024;
     static_assert(STAGE_BYTES % 1024 == 0 && TOTAL <= 227 * 1024);
+    static_assert(BM * BN * 4 <= OFF_STAGING); // a split tile's sums, over the ring
 };
 
-struct NoMaps {};
+// Destination of the tiles: q/k/v one map per rank that owns heads (dim, q/k/v x head slot, row), else m[0] (column, row).
+// Boxes are an epilogue warp's 32 rows of 128 bytes.
 template <Epi EPI>
-using MapsOf = std::conditional_t<staged(EPI), OutMaps, NoMaps>;
+struct Fp4Maps {
+    CUtensorMap m[EPI == Epi::qkv ? 8 : 1];
+};
 
 // D[tmem] (+)= A[smem] B[smem]^T on e2m1 codes, the block scales in TMEM at sfa and sfb.
 template <Fp4 F>
@@ -74,246 +86,260 @@ __device__ __forceinline__ constexpr uint32_t idesc_fp4(uint32_t pair)
            (pair << 29);
 }
 
-// One scale tile (32 rows of 16 bytes in shared memory) into four TMEM columns of 32 lanes, repeated for the four
-// 32-lane quarters.
-__device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t smem_addr)
+// The scale copies and MMAs of one stage: `tiles` scale tiles along K and `steps` MMAs (constants in full stages, so that
+// the loops unroll). Scale tile k of A goes to columns tsf + 12 k, of B's two row halves to the next four and four.
+template <Fp4 F>
+__device__ __forceinline__ void issue_stage(uint32_t d, uint64_t ad, uint64_t bd, uint64_t fd, uint32_t tsf, int tiles, int steps, bool fresh)
 {
-    // 8-row groups of 128 bytes, no swizzle
-    const uint64_t d = uint64_t((smem_addr >> 4) & 0x3FFF) | (uint64_t(128 >> 4) << 32) | (uint64_t(1) << 46);
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
-}
-
-// `CHUNKS` 32-column chunks of this thread's accumulator row, from column `col`, as they are.
-template <int CHUNKS>
-__device__ __forceinline__ void load_chunks(uint32_t taddr, int col, float* v)
-{
-    uint32_t r[CHUNKS][32];
+    constexpr int KT = Fp4Smem<F>::KT;
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c)
-        tmem_ld32(taddr + col + c * 32, r[c]);
-    tmem_wait_ld();
+    for (int k = 0; k < tiles; ++k)
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c)
+        for (int x = 0; x < 3; ++x)
+            // one tile, 32 rows of 16 bytes, into four columns of 32 lanes, repeated for the four lane quarters
+            asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tsf + k * 12 + x * 4), "l"(fd + (x * KT + k) * (512 >> 4))
+                         : "memory");
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-            v[c * 32 + i] = __uint_as_float(r[c][i]);
-}
-
-// 32 columns from `col` times the row scales, plus the bias. Columns past N (whole groups of 8) are left alone.
-__device__ __forceinline__ void finish_chunk(const GemmParams& p, float* v, int col, float a_scale)
-{
-    if (p.b_scale) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (col + 4 * i < p.N) {
-                const float4 b = __ldg(reinterpret_cast<const float4*>(p.b_scale + col) + i);
-                v[4 * i] *= a_scale * b.x, v[4 * i + 1] *= a_scale * b.y, v[4 * i + 2] *= a_scale * b.z, v[4 * i + 3] *= a_scale * b.w;
-            }
-    } else if (p.a_scale) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-            v[i] *= a_scale;
-    }
-    if (p.bias) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (col + 4 * i < p.N) {
-                const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + col) + i);
-                v[4 * i] += b.x, v[4 * i + 1] += b.y, v[4 * i + 2] += b.z, v[4 * i + 3] += b.w;
-            }
+    for (int k = 0; k < steps; ++k) {
+        const uint32_t sf = tsf + (F == Fp4::nv ? k : k / 2) * 12;
+        mma_fp4<F>(d, ad + k * (32 >> 4), bd + k * (32 >> 4), idesc_fp4<F>(F == Fp4::nv ? 0 : (k & 1) * 2), sf, sf + 4, !fresh || k > 0);
     }
 }
 
-// The output of 32 finished columns of row gm (bf16, f32 and gated residual epilogues).
+__device__ __forceinline__ void tma_reduce_add_2d(const void* tmap, const void* smem_src, int32_t c0, int32_t c1)
+{
+    asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                     reinterpret_cast<uint64_t>(tmap)),
+                 "r"(smem_u32(smem_src)), "r"(c0), "r"(c1)
+                 : "memory");
+}
+
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr, uint32_t rank)
+{
+    float4 v;
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\tld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr), "r"(rank)
+                 : "memory");
+    return v;
+}
+
+// g / (1 + e^-g); the quotient within 2 ulp (0 once e^-g is above 2^126, where it is below 2^-119)
+__device__ __forceinline__ float silu_approx(float g) { return __fdividef(g, 1.0f + __expf(-g)); }
+
+// First of the columns [half 0: 0, half 1: 64) ... that an epilogue thread's 32-column chunk c of 4 holds, within the tile. The
+// SwiGLU pairs gate column j with value column 128 + j, so a thread takes 64 of both; else 128 columns in a row.
 template <Epi EPI>
-__device__ __forceinline__ void store_chunk(const GemmParams& p, const float* v, int gm, int col)
+__device__ __forceinline__ int chunk_col(int half, int c)
 {
-    if constexpr (EPI == Epi::bf16) {
-        uint4* d = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + size_t(gm) * p.ldo + col);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (col + 8 * i < p.N)
-                d[i] = make_uint4(pack_bf16x2(v[8 * i], v[8 * i + 1]), pack_bf16x2(v[8 * i + 2], v[8 * i + 3]),
-                                  pack_bf16x2(v[8 * i + 4], v[8 * i + 5]), pack_bf16x2(v[8 * i + 6], v[8 * i + 7]));
-    } else if constexpr (EPI == Epi::f32) {
-        float4* d = reinterpret_cast<float4*>(static_cast<float*>(p.out) + size_t(gm) * p.ldo + col);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (col + 4 * i < p.N)
-                d[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-    } else {
-        static_assert(EPI == Epi::gate_resid);
-        const float4* g4 = reinterpret_cast<const float4*>(p.mod + (size_t(p.mod_idx[gm]) * 6 + p.gate_slot) * p.dim + col);
-        float4* x4 = reinterpret_cast<float4*>(p.x + size_t(gm) * p.ldx + col);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (col + 4 * i < p.N) {
-                const float4 g = __ldg(g4 + i);
-                float4 x = x4[i];
-                x.x += g.x * v[4 * i], x.y += g.y * v[4 * i + 1], x.z += g.z * v[4 * i + 2], x.w += g.w * v[4 * i + 3];
-                x4[i] = x;
-            }
-    }
+    return EPI == Epi::swiglu ? half * 64 + (c >> 1) * 128 + (c & 1) * 32 : half * 128 + c * 32;
 }
 
-// Sixteen-byte piece `c` (8 columns) of a row's 128 staged bf16 columns (two 128-byte-swizzled halves).
-__device__ __forceinline__ void stage_piece(uint8_t* stage, int row, int c, const float* v)
+// Piece `i` (16 bytes) of this lane's 128-byte row of the warp's staging buffer, swizzled as the tensor map has it.
+__device__ __forceinline__ void stage_piece(uint8_t* buf, int i, uint4 v) { *reinterpret_cast<uint4*>(buf + lane_id() * 128 + ((i ^ (lane_id() & 7)) << 4)) = v; }
+__device__ __forceinline__ uint4 pack8(const float* v)
 {
-    *reinterpret_cast<uint4*>(stage + (c >> 3) * (BM * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
-        make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+    return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
 
-// The epilogue of one tile whose accumulator is number ACC. The columns that the other accumulator shares (the last 96 of
-// accumulator 0, the first 96 of accumulator 1) are read first; `release` then lets the next tile's MMAs start.
-template <Epi EPI, int ACC, class Release>
-__device__ __forceinline__ void epilogue_fp4(const GemmParams& p, uint32_t tmem, int m0, int n0, uint8_t* stage, const MapsOf<EPI>& om,
-                                             Release&& release)
+// The epilogue of this warp's 32 rows x 128 columns: takes the accumulator (release() once it is in registers), then 4 KB
+// of finished output at a time through the warp's staging buffer, stored by TMA (which clips rows past M and columns past
+// N). cols: the columns' row scales of B, then their biases.
+template <Epi EPI, class Release>
+__device__ __forceinline__ void epilogue_fp4(const GemmParams& p, uint32_t taddr, int m0, int n0, int half, uint8_t* buf, const float* cols,
+                                             const Fp4Maps<EPI>& om, Release&& release)
 {
-    constexpr int FIRST = ACC == 0 ? ACC1 : 0; // first shared column of this accumulator
-    const int quarter = warp_id() & 3;
-    const int row = quarter * 32 + lane_id();
-    const int gm = m0 + row;
+    const int gm = m0 + lane_id(); // m0: the warp's first row
     const bool valid = gm < p.M;
-    const uint32_t taddr = tmem + (ACC == 0 ? 0 : ACC1) + (uint32_t(quarter * 32) << 16);
     const float a_scale = p.a_scale && valid ? __ldg(p.a_scale + gm) : 1.0f;
-
-    if constexpr (EPI == Epi::qkv) {
-        const int sec = n0 / p.inner;
-        const int grow = valid ? gm : p.M - 1; // rows past M read a valid row's rotary entry
-#pragma unroll 1
-        for (int i = 0; i < 2; ++i) {
-            const int hh = ACC == 0 ? 1 - i : i; // the head that lies in the shared columns first
-            float v[128];
-            load_chunks<4>(taddr, hh * 128, v);
-            if (i == 0)
-                release();
-            const int col = n0 + hh * 128;
+    float v[128];
+    {
+        uint32_t r[4][32];
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-                finish_chunk(p, v + 32 * c, col + 32 * c, a_scale);
-            if (sec < 2) {
-                float ss = 0.f;
-#pragma unroll
-                for (int j = 0; j < 128; ++j)
-                    ss += v[j] * v[j];
-                const float rinv = rsqrtf(ss * (1.0f / 128.0f) + p.eps);
-                const float* w = sec == 0 ? p.qn_w : p.kn_w;
-#pragma unroll
-                for (int j = 0; j < 128; ++j)
-                    v[j] = v[j] * rinv * __ldg(w + j);
-                const float2* cs = reinterpret_cast<const float2*>(p.rope) + size_t(grow) * 48;
-#pragma unroll
-                for (int j = 0; j < 48; ++j) {
-                    const float2 t = __ldg(cs + j);
-                    const float a = v[j], b = v[j + 48];
-                    v[j] = a * t.x - b * t.y;
-                    v[j + 48] = b * t.x + a * t.y;
-                }
-            }
-            const int head = (col % p.inner) / 128;
-            const int rank = head / p.heads_per_rank, hl = head % p.heads_per_rank;
-            if (threadIdx.x == 64)
-                bulk_wait_read0(); // the staged tile before has been read
-            epi_bar();
-#pragma unroll
-            for (int c = 0; c < 16; ++c)
-                stage_piece(stage, row, c, v + 8 * c);
-            fence_proxy_async_smem();
-            epi_bar();
-            if (threadIdx.x == 64) {
-                const int slot = sec * p.heads_per_rank + hl;
-                tma_store_3d(&om.m[rank], stage, 0, slot, m0);
-                tma_store_3d(&om.m[rank], stage + BM * 128, 64, slot, m0);
-                bulk_commit();
-            }
-        }
-    } else if constexpr (EPI == Epi::swiglu) {
-        // pair c: gate chunk c and value chunk c + 4; the shared columns hold the values of pairs 1..3 (accumulator 0) or the
-        // gates of pairs 0..2 (accumulator 1)
-        float held[OVERLAP];
-        load_chunks<3>(taddr, FIRST, held);
+        for (int c = 0; c < 4; ++c)
+            tmem_ld32(taddr + chunk_col<EPI>(half, c), r[c]);
+        tmem_wait_ld();
         release();
-        if (threadIdx.x == 64)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                v[c * 32 + i] = __uint_as_float(r[c][i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        const float4 s = reinterpret_cast<const float4*>(cols)[i], b = reinterpret_cast<const float4*>(cols + 128)[i];
+        v[4 * i] = fmaf(v[4 * i], a_scale * s.x, b.x), v[4 * i + 1] = fmaf(v[4 * i + 1], a_scale * s.y, b.y);
+        v[4 * i + 2] = fmaf(v[4 * i + 2], a_scale * s.z, b.z), v[4 * i + 3] = fmaf(v[4 * i + 3], a_scale * s.w, b.w);
+    }
+    // ready(): the staging buffer's last store has read it; send(): the warp's rows are in it
+    auto ready = [&] {
+        if (lane_id() == 0)
             bulk_wait_read0();
-        epi_bar();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int c = ACC == 0 ? (i + 1) & 3 : i;
-            float g[32], u[32];
-            if (i < 3) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    (ACC == 0 ? u : g)[j] = held[32 * i + j];
-                load_chunks<1>(taddr, ACC == 0 ? c * 32 : 128 + c * 32, ACC == 0 ? g : u);
-            } else {
-                load_chunks<1>(taddr, c * 32, g);
-                load_chunks<1>(taddr, 128 + c * 32, u);
-            }
-            finish_chunk(p, g, n0 + c * 32, a_scale);
-            finish_chunk(p, u, n0 + 128 + c * 32, a_scale);
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-                g[j] = silu(g[j]) * u[j];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                stage_piece(stage, row, c * 4 + j, g + 8 * j);
-        }
+        __syncwarp();
+    };
+    auto send = [&](auto&& store) {
         fence_proxy_async_smem();
-        epi_bar();
-        if (threadIdx.x == 64) {
-            tma_store_2d(&om.m[0], stage, n0 / 2, m0);
-            tma_store_2d(&om.m[0], stage + BM * 128, n0 / 2 + 64, m0);
+        __syncwarp();
+        if (lane_id() == 0 && m0 < p.M) {
+            store();
             bulk_commit();
         }
-    } else {
-        float held[OVERLAP];
-        load_chunks<3>(taddr, FIRST, held);
-        release();
+    };
+
+    if constexpr (EPI == Epi::qkv) {
+        const int col = n0 + half * 128;
+        const int sec = n0 / p.inner;
+        if (sec < 2) {
+            float ss = 0.f;
 #pragma unroll
-        for (int c = 0; c < 3; ++c) {
-            const int col = n0 + FIRST + c * 32;
-            if (valid && col < p.N) {
-                finish_chunk(p, held + 32 * c, col, a_scale);
-                store_chunk<EPI>(p, held + 32 * c, gm, col);
+            for (int j = 0; j < 128; ++j)
+                ss += v[j] * v[j];
+            const float rinv = rsqrtf(ss * (1.0f / 128.0f) + p.eps);
+            const float* w = sec == 0 ? p.qn_w : p.kn_w;
+#pragma unroll
+            for (int j = 0; j < 128; ++j)
+                v[j] = v[j] * rinv * __ldg(w + j);
+            const float2* cs = reinterpret_cast<const float2*>(p.rope) + size_t(valid ? gm : p.M - 1) * 48;
+#pragma unroll
+            for (int j = 0; j < 48; ++j) {
+                const float2 t = __ldg(cs + j);
+                const float a = v[j], b = v[j + 48];
+                v[j] = a * t.x - b * t.y;
+                v[j + 48] = b * t.x + a * t.y;
             }
         }
-#pragma unroll 1
-        for (int c = 0; c < 5; ++c) {
-            const int at = (ACC == 0 ? 0 : OVERLAP) + c * 32, col = n0 + at;
-            float v[32];
-            load_chunks<1>(taddr, at, v);
-            if (valid && col < p.N) {
-                finish_chunk(p, v, col, a_scale);
-                store_chunk<EPI>(p, v, gm, col);
-            }
+        const int head = (col % p.inner) / 128;
+        const int rank = head / p.heads_per_rank, slot = sec * p.heads_per_rank + head % p.heads_per_rank;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            ready();
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                stage_piece(buf, i, pack8(v + h * 64 + i * 8));
+            send([&] { tma_store_3d(&om.m[rank], buf, h * 64, slot, m0); });
+        }
+    } else if constexpr (EPI == Epi::swiglu) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j)
+            v[j] = silu_approx(v[j]) * v[64 + j];
+        ready();
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            stage_piece(buf, i, pack8(v + i * 8));
+        send([&] { tma_store_2d(&om.m[0], buf, n0 / 2 + half * 64, m0); });
+    } else if constexpr (EPI == Epi::bf16) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            ready();
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                stage_piece(buf, i, pack8(v + h * 64 + i * 8));
+            const int col = n0 + half * 128 + h * 64;
+            send([&] {
+                if (col < p.N)
+                    tma_store_2d(&om.m[0], buf, col, m0);
+            });
+        }
+    } else {
+        // f32 as it is; the gated residual adds gate * v to x where x lies (one fp32 addition per value, by the TMA reduction)
+        if constexpr (EPI == Epi::gate_resid) {
+            const float4* g4 = reinterpret_cast<const float4*>(p.mod + (size_t(valid ? p.mod_idx[gm] : 0) * 6 + p.gate_slot) * p.dim + n0 + half * 128);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (n0 + half * 128 + 4 * i < p.N) {
+                    const float4 g = __ldg(g4 + i);
+                    v[4 * i] *= g.x, v[4 * i + 1] *= g.y, v[4 * i + 2] *= g.z, v[4 * i + 3] *= g.w;
+                }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            ready();
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                stage_piece(buf, i, *reinterpret_cast<const uint4*>(v + c * 32 + i * 4));
+            const int col = n0 + half * 128 + c * 32;
+            send([&] {
+                if (col < p.N) {
+                    if constexpr (EPI == Epi::f32)
+                        tma_store_2d(&om.m[0], buf, col, m0);
+                    else
+                        tma_reduce_add_2d(&om.m[0], buf, col, m0);
+                }
+            });
         }
     }
 }
 
-template <Epi EPI, Fp4 F>
+// Four columns from `col` of row gm of a split tile: the parts' sums (s, and u for the SwiGLU's values at column col + 128)
+// through the epilogue, straight to the output.
+template <Epi EPI>
+__device__ __forceinline__ void finish4(const GemmParams& p, float4 s, float4 u, int gm, int col)
+{
+    const float a = p.a_scale ? __ldg(p.a_scale + gm) : 1.f;
+    auto scaled = [&](float4 v, int c) {
+        const float4 b = p.b_scale ? __ldg(reinterpret_cast<const float4*>(p.b_scale + c)) : make_float4(1.f, 1.f, 1.f, 1.f);
+        const float4 d = p.bias ? __ldg(reinterpret_cast<const float4*>(p.bias + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        return make_float4(fmaf(v.x, a * b.x, d.x), fmaf(v.y, a * b.y, d.y), fmaf(v.z, a * b.z, d.z), fmaf(v.w, a * b.w, d.w));
+    };
+    float4 v = scaled(s, col);
+    if constexpr (EPI == Epi::gate_resid) {
+        const float4 g = __ldg(reinterpret_cast<const float4*>(p.mod + (size_t(p.mod_idx[gm]) * 6 + p.gate_slot) * p.dim + col));
+        float4* x = reinterpret_cast<float4*>(p.x + size_t(gm) * p.ldx + col);
+        float4 o = *x;
+        o.x = __fadd_rn(o.x, v.x * g.x), o.y = __fadd_rn(o.y, v.y * g.y), o.z = __fadd_rn(o.z, v.z * g.z), o.w = __fadd_rn(o.w, v.w * g.w);
+        *x = o;
+    } else if constexpr (EPI == Epi::f32) {
+        *reinterpret_cast<float4*>(static_cast<float*>(p.out) + size_t(gm) * p.ldo + col) = v;
+    } else {
+        int at = col;
+        if constexpr (EPI == Epi::swiglu) {
+            u = scaled(u, col + 128);
+            v = make_float4(silu_approx(v.x) * u.x, silu_approx(v.y) * u.y, silu_approx(v.z) * u.z, silu_approx(v.w) * u.w);
+            at = (col >> 8) * 128 + (col & 127);
+        }
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + size_t(gm) * p.ldo + at) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+    }
+}
+
+// SPLIT: the CTAs of a cluster share one tile's K; else a CTA walks whole tiles.
+template <Epi EPI, Fp4 F, bool SPLIT>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
     gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const uint8_t* a_scales,
-                    const uint8_t* b_scales, const GemmParams p, const __grid_constant__ MapsOf<EPI> om)
+                    const uint8_t* b_scales, const GemmParams p, const __grid_constant__ Fp4Maps<EPI> om)
 {
-    using SM = Fp4Smem<EPI, F>;
-    constexpr int STAGES = SM::STAGES, KT = SM::KT;
+    using SM = Fp4Smem<F>;
+    constexpr int KT = SM::KT;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     uint8_t* smem = smem_raw + (((raw + 1023) & ~1023u) - raw);
-    uint8_t* stage = smem + STAGES * SM::STAGE_BYTES;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(stage + SM::STAGING);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SM::OFF_BAR);
     uint64_t* full = bars;              // [STAGES]
     uint64_t* empty = full + STAGES;    // [STAGES]
     uint64_t* tfull = empty + STAGES;   // [2] an accumulator is complete
-    uint64_t* shared_free = tfull + 2;  // the shared columns of the tile before have been read
-    uint64_t* drain = shared_free + 1;
+    uint64_t* taken = tfull + 2;        // an accumulator is in the epilogue's registers
+    uint64_t* drain = taken + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
 
-    const int warp = warp_id();
+    const int warp = __shfl_sync(0xffffffffu, warp_id(), 0);
     const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN;
     const int num_tiles = tiles_m * tiles_n;
-    const int num_kb = (p.K + KSTAGE - 1) / KSTAGE;
     const int scale_tiles = fp4_scale_tiles(p.K, F);
+    int first_tile = blockIdx.x, tile_step = gridDim.x;
+    int kb0 = 0, kb1 = (p.K + KSTAGE - 1) / KSTAGE; // this CTA's stages of K
+    uint32_t split = 1, part = 0;
+    if constexpr (SPLIT) {
+        asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(split));
+        asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(part));
+        first_tile = blockIdx.x / split, tile_step = num_tiles;
+        const int all = kb1; // every part has a stage: the launch has no more parts than stages
+        kb0 = int(part) * all / int(split), kb1 = (int(part) + 1) * all / int(split);
+    }
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) {
@@ -322,7 +348,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
         for (int i = 0; i < 2; ++i)
             mbar_init(&tfull[i], 1);
-        mbar_init(shared_free, 4);
+        mbar_init(taken, EPI_WARPS);
         mbar_init(drain, 1);
         fence_barrier_init();
     }
@@ -337,15 +363,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 
     if (warp == 0 && elect_one_lane()) {
         // ---------------------------------------------------------------------------------------- producer
-        tma_prefetch_desc(&tmA);
-        tma_prefetch_desc(&tmB);
         uint32_t it = 0;
         bool ok = true;
-        for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+        for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
             int tm, tn;
             tile_coords(tile, tiles_m, tiles_n, tm, tn);
             const bool second = tn * BN + 128 < p.N; // B's second 128 rows have scale tiles
-            for (int kb = 0; kb < num_kb; ++kb, ++it) {
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
                 const int s = it % STAGES;
                 if (!(ok = mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1)))
                     break;
@@ -366,18 +390,21 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         if (ok)
             for (uint32_t j = it >= STAGES ? it - STAGES : 0; j < it; ++j)
                 mbar_wait(&empty[j % STAGES], (j / STAGES) & 1);
-    } else if (warp == 1 && elect_one_lane()) {
+    } else if (warp == 1) {
         // ------------------------------------------------------------------------------------- MMA issuer
+        uint32_t elected;
+        asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
+        const uint32_t smem0 = smem_u32(smem);
         uint32_t it = 0, t_local = 0;
         bool ok = true;
-        for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++t_local) {
-            // the tile before has left the columns that both accumulators use (and, as its epilogue came after that of the
-            // tile before it, this accumulator is free)
-            if (t_local > 0 && !(ok = mbar_wait(shared_free, (t_local - 1) & 1)))
+        for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step, ++t_local) {
+            // the accumulator of the tile before, which shares columns with this one's, has been taken (and this one's own
+            // of two tiles ago before that)
+            if (t_local > 0 && !(ok = mbar_wait(taken, (t_local - 1) & 1)))
                 break;
             tc_fence_after();
             const uint32_t d = tmem + (t_local & 1) * ACC1;
-            for (int kb = 0; kb < num_kb; ++kb, ++it) {
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
                 const int s = it % STAGES;
                 if (!(ok = mbar_wait(&full[s], (it / STAGES) & 1)))
                     break;
@@ -385,84 +412,197 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 if (it >= 2 && !(ok = mbar_wait(&empty[(it - 2) % STAGES], ((it - 2) / STAGES) & 1)))
                     break;
                 tc_fence_after();
-                const uint32_t sa = smem_u32(smem + s * SM::STAGE_BYTES);
-                const uint32_t sb = sa + A_BYTES, sf = sb + B_BYTES;
+                const uint32_t sa = smem0 + s * SM::STAGE_BYTES, sf = sa + A_BYTES + B_BYTES;
+                const uint64_t ad = sdesc_sw128(sa, 16, 1024), bd = sdesc_sw128(sa + A_BYTES, 16, 1024);
+                // scale tiles: 8-row groups of 128 bytes, no swizzle
+                const uint64_t fd = uint64_t((sf >> 4) & 0x3FFF) | (uint64_t(128 >> 4) << 32) | (uint64_t(1) << 46);
                 const uint32_t tsf = tmem + SCALE_COL + (it & 1) * SCALE_BUF;
-                const int steps = min(KSTAGE, p.K - kb * KSTAGE + 63) / 64; // MMAs of this stage (64 values each)
-                const int kts = min(KT, scale_tiles - kb * KT);
-                for (int k = 0; k < kts; ++k) {
-                    copy_scales(tsf + k * 12, sf + k * 512);
-                    copy_scales(tsf + k * 12 + 4, sf + (KT + k) * 512);
-                    copy_scales(tsf + k * 12 + 8, sf + (2 * KT + k) * 512);
+                const int left = p.K - kb * KSTAGE;
+                if (elected) {
+                    if (left >= KSTAGE)
+                        issue_stage<F>(d, ad, bd, fd, tsf, KT, KSTAGE / 64, kb == kb0);
+                    else
+                        issue_stage<F>(d, ad, bd, fd, tsf, scale_tiles - kb * KT, (left + 63) / 64, kb == kb0);
+                    mma_commit(&empty[s]);
                 }
-#pragma unroll
-                for (int k = 0; k < KSTAGE / 64; ++k) {
-                    if (k >= steps)
-                        break;
-                    const uint64_t ad = sdesc_sw128(sa + k * 32, 16, 1024);
-                    const uint64_t bd = sdesc_sw128(sb + k * 32, 16, 1024);
-                    const uint32_t kt = F == Fp4::nv ? k : k / 2;
-                    mma_fp4<F>(d, ad, bd, idesc_fp4<F>(F == Fp4::nv ? 0 : (k & 1) * 2), tsf + kt * 12, tsf + kt * 12 + 4, (kb | k) != 0);
-                }
-                mma_commit(&empty[s]);
+                __syncwarp();
             }
-            if (ok)
+            if (ok && elected)
                 mma_commit(&tfull[t_local & 1]);
+            __syncwarp();
         }
-        // Every MMA this thread issued has completed once `drain` flips.
-        mma_commit(drain);
+        // Every MMA this warp issued has completed once `drain` flips.
+        if (elected)
+            mma_commit(drain);
+        __syncwarp();
         mbar_wait(drain, 0);
     } else if (warp >= 2) {
         // ---------------------------------------------------------------------------------------- epilogue
-        uint32_t t_local = 0;
-        auto release = [&] {
-            tc_fence_before();
-            __syncwarp();
-            if (elect_one_lane())
-                mbar_arrive(shared_free);
-        };
-        for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x, ++t_local) {
-            const int acc = t_local & 1;
-            if (!mbar_wait(&tfull[acc], (t_local >> 1) & 1))
-                break;
-            tc_fence_after();
+        const int quarter = warp & 3, half = (warp - 2) >> 2; // its 32 TMEM lanes, its half of the columns
+        const uint32_t lanes = uint32_t(quarter * 32) << 16;
+        if constexpr (SPLIT) {
+            // This part's sums, rows below M only: row r's 16-byte piece i at (i ^ (r & 7)), over the ring (its loads have
+            // been read by the MMAs that `tfull` follows).
             int tm, tn;
-            tile_coords(tile, tiles_m, tiles_n, tm, tn);
-            if (acc == 0)
-                epilogue_fp4<EPI, 0>(p, tmem, tm * BM, tn * BN, stage, om, release);
-            else
-                epilogue_fp4<EPI, 1>(p, tmem, tm * BM, tn * BN, stage, om, release);
+            tile_coords(first_tile, tiles_m, tiles_n, tm, tn);
+            const int r = quarter * 32 + lane_id();
+            if (mbar_wait(&tfull[0], 0)) {
+                tc_fence_after();
+                if (tm * BM + quarter * 32 < p.M) {
+                    float4* row = reinterpret_cast<float4*>(smem) + r * (BN / 4);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t o[32];
+                        tmem_ld32(tmem + lanes + half * 128 + c * 32, o);
+                        tmem_wait_ld();
+                        if (tm * BM + r < p.M)
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                row[(half * 32 + c * 8 + i) ^ (r & 7)] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                                                                     __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+                    }
+                }
+            }
+        } else {
+            uint8_t* buf = smem + SM::OFF_STAGING + (warp - 2) * 4096;
+            float* cols = reinterpret_cast<float*>(smem + SM::OFF_COLS) + (warp - 2) * 256;
+            auto release = [&] {
+                tc_fence_before();
+                __syncwarp();
+                if (elect_one_lane())
+                    mbar_arrive(taken);
+            };
+            uint32_t t_local = 0;
+            for (int tile = first_tile; tile < num_tiles; tile += tile_step, ++t_local) {
+                const int acc = t_local & 1;
+                int tm, tn;
+                tile_coords(tile, tiles_m, tiles_n, tm, tn);
+                {
+                    // the columns' scales and biases, four a lane, while the MMAs run
+                    const int j = lane_id() * 4, col = tn * BN + chunk_col<EPI>(half, j >> 5) + (j & 31);
+                    const float4 one = make_float4(1.f, 1.f, 1.f, 1.f), none = make_float4(0.f, 0.f, 0.f, 0.f);
+                    reinterpret_cast<float4*>(cols)[lane_id()] = p.b_scale && col < p.N ? __ldg(reinterpret_cast<const float4*>(p.b_scale + col)) : one;
+                    reinterpret_cast<float4*>(cols + 128)[lane_id()] = p.bias && col < p.N ? __ldg(reinterpret_cast<const float4*>(p.bias + col)) : none;
+                    __syncwarp();
+                }
+                if (!mbar_wait(&tfull[acc], (t_local >> 1) & 1))
+                    break;
+                tc_fence_after();
+                epilogue_fp4<EPI>(p, tmem + lanes + acc * ACC1, tm * BM + quarter * 32, tn * BN, half, buf, cols, om, release);
+                __syncwarp(); // every lane has read `cols`
+            }
+            if (lane_id() == 0)
+                bulk_wait0(); // the staged tiles' stores are complete
         }
-        if (staged(EPI) && threadIdx.x == 64)
-            bulk_wait0(); // the staged tiles' TMA stores are complete
     }
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
+    if constexpr (SPLIT) {
+        // The tile's rows below M in groups of four columns (SwiGLU: of outputs), dealt out over the cluster's threads.
+        cluster_sync();
+        int tm, tn;
+        tile_coords(first_tile, tiles_m, tiles_n, tm, tn);
+        constexpr int GROUPS = EPI == Epi::swiglu ? BN / 8 : BN / 4;
+        const int rows = min(BM, p.M - tm * BM);
+        for (int i = int(part) * NUM_THREADS + threadIdx.x; i < rows * GROUPS; i += int(split) * NUM_THREADS) {
+            const int r = i / GROUPS, g = i % GROUPS, col = tn * BN + g * 4;
+            if (col >= p.N)
+                continue;
+            auto sum = [&](int piece) {
+                const uint32_t at = smem_u32(smem) + (r * (BN / 4) + (piece ^ (r & 7))) * 16;
+                float4 s = ld_cluster4(at, 0);
+                for (uint32_t z = 1; z < split; ++z) {
+                    const float4 v = ld_cluster4(at, z);
+                    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+                }
+                return s;
+            };
+            const float4 s = sum(g);
+            finish4<EPI>(p, s, EPI == Epi::swiglu ? sum(g + 32) : s, tm * BM + r, col);
+        }
+        cluster_sync(); // no CTA leaves while another reads its shared memory
+    }
 }
 
-template <Epi EPI, Fp4 F>
-void launch(const void* A, const void* a_scales, const void* B, const void* b_scales, const GemmParams& p, cudaStream_t s)
+template <Epi EPI>
+Fp4Maps<EPI> output_maps(const GemmParams& p)
 {
-    using SM = Fp4Smem<EPI, F>;
+    Fp4Maps<EPI> om{};
+    if constexpr (EPI == Epi::qkv) {
+        const int P = p.inner / 128 / p.heads_per_rank;
+        const uint64_t slots = 3 * uint64_t(p.heads_per_rank);
+        const uint64_t dims[3] = {128, slots, uint64_t(p.M)}, pitch[2] = {256, slots * 256};
+        const uint32_t box[3] = {64, 1, 32};
+        for (int r = 0; r < P; ++r)
+            om.m[r] = make_tmap(CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, static_cast<const __nv_bfloat16*>(p.out) + size_t(r) * p.rows_local * slots * 128, dims,
+                                pitch, box);
+    } else {
+        constexpr bool wide = EPI == Epi::f32 || EPI == Epi::gate_resid;
+        const int64_t ld = EPI == Epi::gate_resid ? p.ldx : p.ldo;
+        const uint64_t n = EPI == Epi::swiglu ? p.N / 2 : p.N, size = wide ? 4 : 2;
+        const uint64_t dims[2] = {n, uint64_t(p.M)}, pitch[1] = {(p.M > 1 ? uint64_t(ld) : (n + 7) / 8 * 8) * size};
+        const uint32_t box[2] = {wide ? 32u : 64u, 32};
+        om.m[0] = make_tmap(wide ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                            EPI == Epi::gate_resid ? static_cast<const void*>(p.x) : p.out, dims, pitch, box);
+    }
+    return om;
+}
+
+template <Epi EPI, Fp4 F, bool SPLIT>
+bool launch(const void* A, const void* a_scales, const void* B, const void* b_scales, const GemmParams& p, int tiles, int ctas, cudaStream_t s)
+{
+    using SM = Fp4Smem<F>;
     const uint64_t bytes = uint64_t(p.K) / 2;
     const uint64_t adims[2] = {bytes, uint64_t(p.M)}, bdims[2] = {bytes, uint64_t(p.N)}, pitch[1] = {bytes};
     const uint32_t abox[2] = {128, BM}, bbox[2] = {128, BN};
     const CUtensorMap ta = make_tmap(CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, A, adims, pitch, abox);
     const CUtensorMap tb = make_tmap(CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, B, bdims, pitch, bbox);
-    MapsOf<EPI> om{};
-    if constexpr (staged(EPI))
-        om = out_maps<EPI>(p, p.M);
+    Fp4Maps<EPI> om{};
+    if constexpr (!SPLIT)
+        om = output_maps<EPI>(p);
     static std::atomic<uint64_t> opt_in;
-    smem_opt_in(gemm_fp4_kernel<EPI, F>, SM::TOTAL, opt_in);
+    smem_opt_in(gemm_fp4_kernel<EPI, F, SPLIT>, SM::TOTAL, opt_in);
+    cudaLaunchConfig_t c{};
+    c.blockDim = dim3(NUM_THREADS);
+    c.dynamicSmemBytes = SM::TOTAL;
+    c.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    c.attrs = at;
+    int split = 1;
+    if constexpr (SPLIT) {
+        // the largest cluster of which the device holds one per tile at once, with a stage for every CTA
+        c.numAttrs = 1;
+        static ClusterLimits limits;
+        for (split = std::min({ctas / tiles, MAX_SPLIT, (p.K + KSTAGE - 1) / KSTAGE}); split > 1; --split)
+            if (limits.at_once(gemm_fp4_kernel<EPI, F, true>, c, split) >= tiles)
+                break;
+        if (split < 2)
+            return false;
+        at[0].val.clusterDim.x = unsigned(split);
+        ctas = tiles * split;
+    }
+    c.gridDim = dim3(unsigned(ctas));
+    H3_CUDA(cudaLaunchKernelEx(&c, gemm_fp4_kernel<EPI, F, SPLIT>, ta, tb, static_cast<const uint8_t*>(a_scales),
+                               static_cast<const uint8_t*>(b_scales), p, om));
+    return true;
+}
+
+template <Epi EPI, Fp4 F>
+void run(const void* A, const void* a_scales, const void* B, const void* b_scales, const GemmParams& p, cudaStream_t s)
+{
     const long long tiles = (long long)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
-    const int grid = int(std::min<long long>(tiles, num_sms()));
-    gemm_fp4_kernel<EPI, F><<<grid, NUM_THREADS, SM::TOTAL, s>>>(ta, tb, static_cast<const uint8_t*>(a_scales),
-                                                                 static_cast<const uint8_t*>(b_scales), p, om);
-    H3_CUDA(cudaGetLastError());
+    const int sms = num_sms();
+    if constexpr (EPI != Epi::qkv) // its norm runs along whole rows of a tile
+        if (tiles * 2 <= sms && p.K > KSTAGE && launch<EPI, F, true>(A, a_scales, B, b_scales, p, int(tiles), sms, s))
+            return;
+    launch<EPI, F, false>(A, a_scales, B, b_scales, p, int(tiles), int(std::min<long long>(tiles, sms)), s);
 }
 
 } // namespace
@@ -474,11 +614,11 @@ void gemm_fp4(const void* A, const void* a_scales, const void* B, const void* b_
         return;
     const bool nv = f == Fp4::nv;
     switch (epi) {
-    case Epi::bf16: return (nv ? launch<Epi::bf16, Fp4::nv> : launch<Epi::bf16, Fp4::mx>)(A, a_scales, B, b_scales, p, s);
-    case Epi::f32: return (nv ? launch<Epi::f32, Fp4::nv> : launch<Epi::f32, Fp4::mx>)(A, a_scales, B, b_scales, p, s);
-    case Epi::qkv: return (nv ? launch<Epi::qkv, Fp4::nv> : launch<Epi::qkv, Fp4::mx>)(A, a_scales, B, b_scales, p, s);
-    case Epi::gate_resid: return (nv ? launch<Epi::gate_resid, Fp4::nv> : launch<Epi::gate_resid, Fp4::mx>)(A, a_scales, B, b_scales, p, s);
-    case Epi::swiglu: return (nv ? launch<Epi::swiglu, Fp4::nv> : launch<Epi::swiglu, Fp4::mx>)(A, a_scales, B, b_scales, p, s);
+    case Epi::bf16: return (nv ? run<Epi::bf16, Fp4::nv> : run<Epi::bf16, Fp4::mx>)(A, a_scales, B, b_scales, p, s);
+    case Epi::f32: return (nv ? run<Epi::f32, Fp4::nv> : run<Epi::f32, Fp4::mx>)(A, a_scales, B, b_scales, p, s);
+    case Epi::qkv: return (nv ? run<Epi::qkv, Fp4::nv> : run<Epi::qkv, Fp4::mx>)(A, a_scales, B, b_scales, p, s);
+    case Epi::gate_resid: return (nv ? run<Epi::gate_resid, Fp4::nv> : run<Epi::gate_resid, Fp4::mx>)(A, a_scales, B, b_scales, p, s);
+    case Epi::swiglu: return (nv ? run<Epi::swiglu, Fp4::nv> : run<Epi::swiglu, Fp4::mx>)(A, a_scales, B, b_scales, p, s);
     default: throw std::runtime_error("gemm_fp4: unsupported epilogue");
     }
 }
