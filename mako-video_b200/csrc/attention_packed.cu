@@ -13,8 +13,10 @@
 //   - Keys come as the prefix's 128-row blocks, then the document's own (one run where they adjoin). Rows of a block past
 //     its end belong to someone else and may hold anything: their scores are replaced, and their V rows are zeroed in
 //     shared memory (0 x NaN is a NaN) by tile 0's softmax warps before they hand over P.
-//   - With few runs the keys are split over the CTAs of a cluster, and the parts joined through shared memory of the
-//     cluster: no scratch in HBM, no second launch, a fixed order of the sums.
+//   - A run that fills one tile only has its even key blocks in one tile's place and its odd ones in the other's, so that
+//     the two still overlap (a row's keys then come in two parts).
+//   - With few runs the keys are split over the CTAs of a cluster. Parts are joined through the cluster's shared memory: no
+//     scratch in HBM, no second launch, a fixed order of the sums.
 #include "attention_packed.cuh"
 #include "common.hpp"
 #include "ptx.cuh"
@@ -29,8 +31,11 @@ namespace {
 
 constexpr int HALF = 16384;                // 128 rows x 64 dims of 2 bytes
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
-constexpr int KST = 3, VST = 2;            // K is freed once both S MMAs read it, V after both PV MMAs
+// K and V slots. K is freed once its S MMAs have read it, V after its PV MMAs. With one query tile its room for a second
+// one is a third V slot.
+constexpr int KST = 3, VST = 2;
 constexpr int NT = 64 + 256;
+constexpr int LEAST = 4; // 128-key blocks that a CTA takes before another one joins it
 
 template <int HD>
 struct PkSmem {
@@ -73,6 +78,19 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi)
     }
 }
 
+// -infinity in this warp's lanes of the TMEM columns [from, 128) after `taddr`. (Masking the scores in registers instead
+// costs every step their spills.)
+__device__ __forceinline__ void hide_columns(uint32_t taddr, int from)
+{
+    const uint32_t inf = 0xff800000u;
+    int c = from;
+    for (; c & 7; ++c)
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr + c), "r"(inf));
+    for (; c < 128; c += 8)
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %1, %1, %1, %1, %1, %1, %1};" ::"r"(taddr + c), "r"(inf));
+    tmem_wait_st();
+}
+
 __device__ __forceinline__ void cluster_sync()
 {
     asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
@@ -98,27 +116,378 @@ __device__ __forceinline__ float2 ld_cluster2(uint32_t addr, uint32_t rank)
     return v;
 }
 
-// The document whose slots hold `slot`, or -1: the last d with q_start[d] / run + d <= slot. One warp, 32 candidates a step.
-__device__ __forceinline__ int find_document(const PkArgs& p, int slot, int run)
+struct Document {
+    int index, q0, q1, k0, k1;
+};
+
+// The document whose slots hold `slot`: the last d with q_start[d] / run + d <= slot (index -1: none). One warp, 32
+// candidates a step; the last step has read the starts by the time it knows which it needs.
+__device__ __forceinline__ Document find_document(const PkArgs& p, int slot, int run)
 {
     int lo = 0, n = p.docs;
     while (true) {
         const int step = (n + 31) / 32;
-        const int d = lo + lane_id() * step;
-        const bool before = lane_id() * step < n && min(max(__ldg(p.q_start + d), 0), p.q_rows) / run + d <= slot;
-        const uint32_t yes = __ballot_sync(0xffffffffu, before);
-        if (!yes)
-            return -1; // rows before the first document
-        const int k = 31 - __clz(yes);
+        const bool in = lane_id() * step < n;
+        const int d = lo + (in ? lane_id() * step : 0);
+        const int q0 = __ldg(p.q_start + d), q1 = __ldg(p.q_start + d + 1), k0 = __ldg(p.k_start + d), k1 = __ldg(p.k_start + d + 1);
+        const uint32_t yes = __ballot_sync(0xffffffffu, in && min(max(q0, 0), p.q_rows) / run + d <= slot);
+        const int k = yes ? 31 - __clz(yes) : 0;
+        if (!yes || step == 1) {
+            Document r;
+            r.index = yes ? lo + k : -1; // -1: rows before the first document
+            r.q0 = __shfl_sync(0xffffffffu, q0, k), r.q1 = __shfl_sync(0xffffffffu, q1, k);
+            r.k0 = __shfl_sync(0xffffffffu, k0, k), r.k1 = __shfl_sync(0xffffffffu, k1, k);
+            return r;
+        }
         lo += k * step;
         n = min(step, n - k * step);
-        if (step == 1)
-            return lo;
     }
 }
 
+// The run of `run_rows` query rows that a slot is, and the keys that they see.
+struct Run {
+    int row0, q1;             // query rows [row0, q1) (q1: the document's end)
+    int a_end, b0, b_end;     // keys [0, a_end) and [b0, b_end)
+    bool any;
+};
+
+__device__ __forceinline__ Run run_of(const PkArgs& p, int slot, int run_rows)
+{
+    const Document doc = find_document(p, slot, run_rows);
+    Run r;
+    r.row0 = doc.q0 + (slot - (doc.q0 / run_rows + doc.index)) * run_rows, r.q1 = doc.q1;
+    r.any = !(doc.index < 0 || doc.q0 < 0 || r.row0 < doc.q0 || r.row0 >= r.q1 || r.q1 > p.q_rows || doc.k0 < 0 || doc.k1 < doc.k0 ||
+              doc.k1 > p.k_rows);
+    r.a_end = p.prefix;
+    r.b0 = max(doc.k0, p.prefix);
+    r.b_end = max(doc.k1, r.b0);
+    if (r.b0 == p.prefix)
+        r.a_end = r.b_end, r.b0 = r.b_end; // the document's keys adjoin the prefix: one run of keys
+    return r;
+}
+
+// The starts ascend within the tensors; what else they say is a device error, and such documents are left out.
+__device__ __forceinline__ void check_starts(const PkArgs& p, int threads)
+{
+    for (int d = threadIdx.x; d <= p.docs; d += threads) {
+        const int a = p.q_start[d], b = p.k_start[d];
+        if (a < 0 || a > p.q_rows || b < 0 || b > p.k_rows || (d > 0 && (a < p.q_start[d - 1] || b < p.k_start[d - 1])))
+            record_error(kErrBadShape);
+    }
+}
+
+__device__ __forceinline__ void cluster_place(uint32_t& split, uint32_t& part)
+{
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(split));
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(part));
+}
+
+// How many of a cluster's `most` CTAs share a run of `blocks` key blocks: one for every `least`, so that long documents are
+// split further than short ones.
+__device__ __forceinline__ uint32_t parts_of(int blocks, int least, uint32_t most)
+{
+    return min(most, uint32_t(max(1, (blocks + least - 1) / least)));
+}
+
+// ------------------------------------------------------------------------------------------------------------
+// Few rows: 16 / group query rows of a document (16 stacked rows), where the keys' bytes are what counts. A 128-row tile of
+// the tensor core would be nearly empty and, at 1400 clocks for 128 keys, slower than HBM; the warp-wide m16n8k16 MMA fits
+// the rows. Warp 0 streams 64-key blocks of K and V through a ring (TMA); warps 1..4 take 16 keys of each block, with a
+// maximum, a sum and an output of their own (no exchange until the end). Two CTAs an SM.
+//   S (16 x 16) = Q K^T: Q's fragments in registers, K's by ldmatrix; P stays in registers (an MMA's sums are the next one's
+//   A fragment); O (16 x HD) += P V, V's fragments by ldmatrix.trans. Keys past a block's end get -infinity and V 0.
+// The warps' and then the cluster's parts are joined in a fixed order.
+constexpr int FEW_ROWS = 16, FEW_KEYS = 64, FEW_STAGES = 3, FEW_WARPS = 4, FEW_NT = 32 + 32 * FEW_WARPS, FEW_SPLIT = 16;
+constexpr int FEW_LEAST = 16; // blocks that a CTA takes before another one joins it: about 8 us against 7 of starting and joining
+
+template <int HD>
+struct FewSmem {
+    static constexpr int TL = FEW_KEYS * HD * 2; // a block's K, and its V
+    static constexpr int OFF_ML = FEW_STAGES * 2 * TL;              // (max, sum) of the warps' rows, then of the CTA's
+    static constexpr int OFF_BAR = OFF_ML + (FEW_WARPS + 1) * FEW_ROWS * 8;
+    static constexpr int TOTAL = OFF_BAR + 128 + 1024;
+    // the warps' outputs, then the CTA's, over the ring
+    static_assert((FEW_WARPS + 1) * FEW_ROWS * HD * 4 <= FEW_STAGES * 2 * TL);
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+template <bool F16>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    if constexpr (F16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
 template <int HD, bool F16>
-__global__ void __launch_bounds__(NT, 1) packed_attention_kernel(const __grid_constant__ PkMaps maps, const PkArgs p)
+__global__ void __launch_bounds__(FEW_NT, 2) few_rows_kernel(const __grid_constant__ PkMaps maps, const PkArgs p, const void* q, int64_t q_stride)
+{
+    using SM = FewSmem<HD>;
+    constexpr int TL = SM::TL;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    uint8_t* smem = smem_raw + (((raw + 1023) & ~1023u) - raw);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + SM::OFF_BAR); // [FEW_STAGES]
+    uint64_t* empty = full + FEW_STAGES;                              // [FEW_STAGES]
+
+    const int warp = warp_id(), lane = lane_id();
+    uint32_t split, part;
+    cluster_place(split, part);
+    const int kv_head = blockIdx.y, run_rows = FEW_ROWS / p.group;
+    if (blockIdx.x == 0 && blockIdx.y == 0)
+        check_starts(p, FEW_NT);
+    const Run run = run_of(p, blockIdx.x / split, run_rows);
+    if (!run.any)
+        return;
+    const int a_blocks = (run.a_end + FEW_KEYS - 1) / FEW_KEYS;
+    const int blocks = a_blocks + (run.b_end - run.b0 + FEW_KEYS - 1) / FEW_KEYS;
+    split = parts_of(blocks, FEW_LEAST, split);
+    if (part >= split)
+        return; // (a cluster barrier waits for the threads that are left)
+    const int per = (blocks + int(split) - 1) / int(split);
+    const int first = min(int(part) * per, blocks);
+    const int n = min(per, blocks - first);
+    auto block_row = [&](int j) { return first + j < a_blocks ? FEW_KEYS * (first + j) : run.b0 + FEW_KEYS * (first + j - a_blocks); };
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < FEW_STAGES; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], FEW_WARPS);
+        }
+        fence_barrier_init();
+    }
+    __syncthreads();
+
+    const int row_a = lane >> 2, quad = lane & 3; // this thread's stacked rows row_a and row_a + 8, its pair of columns
+    // the query row and head of stacked row r; false: none
+    auto row_of = [&](int r, int& row, int& head) {
+        row = run.row0 + r / p.group, head = kv_head * p.group + r % p.group;
+        return r < run_rows * p.group && row < run.q1;
+    };
+    float o[HD / 8][4];
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < HD / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            o[i][e] = 0.f;
+    bool ok = true;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int j = 0;
+            for (; j < n; ++j) {
+                const int s = j % FEW_STAGES;
+                if (!mbar_wait(&empty[s], ((j / FEW_STAGES) & 1) ^ 1))
+                    break;
+                uint8_t* sk = smem + s * 2 * TL;
+                const int row = block_row(j);
+                mbar_arrive_expect_tx(&full[s], 2 * TL);
+#pragma unroll
+                for (int hh = 0; hh < HD / 64; ++hh) {
+                    tma_load_3d(sk + hh * (FEW_KEYS * 128), &maps.k, &full[s], hh * 64, kv_head, row);
+                    tma_load_3d(sk + TL + hh * (FEW_KEYS * 128), &maps.v, &full[s], hh * 64, kv_head, row);
+                }
+            }
+            // Every load lands before the CTA can exit.
+            for (int i = max(0, j - FEW_STAGES); i < j; ++i)
+                mbar_wait(&full[i % FEW_STAGES], (i / FEW_STAGES) & 1);
+        }
+    } else {
+        uint32_t qf[HD / 16][4];
+        {
+            int row, head;
+            const uint32_t* qa = row_of(row_a, row, head) ? reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(q) + size_t(row) * q_stride + head * HD) : nullptr;
+            const uint32_t* qb = row_of(row_a + 8, row, head) ? reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(q) + size_t(row) * q_stride + head * HD) : nullptr;
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k) {
+                qf[k][0] = qa ? __ldg(qa + k * 8 + quad) : 0, qf[k][2] = qa ? __ldg(qa + k * 8 + 4 + quad) : 0;
+                qf[k][1] = qb ? __ldg(qb + k * 8 + quad) : 0, qf[k][3] = qb ? __ldg(qb + k * 8 + 4 + quad) : 0;
+            }
+        }
+        const int key0 = (warp - 1) * 16; // this warp's keys of a block
+        // ldmatrix addresses: lane i gives row i % 8 of matrix i / 8. K: matrices (keys 0-7, 8 dims), (keys 0-7, next 8), (keys 8-15,
+        // ...), ...; V: (keys 0-7, 8 dims), (keys 8-15, the same), (keys 0-7, next 8), ...
+        const int k_row = key0 + (lane >> 4) * 8 + (lane & 7), k_piece = (lane >> 3) & 1;
+        const int v_row = key0 + ((lane >> 3) & 1) * 8 + (lane & 7), v_piece = lane >> 4;
+        for (int j = 0; j < n; ++j) {
+            const int s = j % FEW_STAGES;
+            if (!(ok = mbar_wait(&full[s], (j / FEW_STAGES) & 1)))
+                break;
+            const int keys = (first + j < a_blocks ? run.a_end : run.b_end) - block_row(j) - key0; // this warp's keys, if under 16
+            if (keys > 0) {
+                const uint32_t sk = smem_u32(smem + s * 2 * TL), sv = sk + TL;
+                float c[2][2][4] = {}; // [k half][key half]: two chains a sum
+#pragma unroll
+                for (int k = 0; k < HD / 16; ++k) {
+                    const int piece = (k & 3) * 2 + k_piece;
+                    uint32_t b[4];
+                    ldmatrix4(b, sk + (k >> 2) * (FEW_KEYS * 128) + k_row * 128 + ((piece ^ (k_row & 7)) << 4));
+                    mma16816<F16>(c[k & 1][0], qf[k], b[0], b[1]);
+                    mma16816<F16>(c[k & 1][1], qf[k], b[2], b[3]);
+                }
+                float sc[2][4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = h * 8 + quad * 2 + (e & 1);
+                        sc[h][e] = key < keys ? c[0][h][e] + c[1][h][e] : -INFINITY;
+                    }
+                float alpha[2];
+                bool need = false;
+#pragma unroll
+                for (int r = 0; r < 2; ++r) { // rows row_a, row_a + 8
+                    float mx = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * p.sl2;
+                    const bool grow = mx > m[r] + kRescaleThreshold;
+                    alpha[r] = grow ? ex2_approx(m[r] - mx) : 1.f;
+                    m[r] = grow ? mx : m[r];
+                    need |= grow;
+                }
+                uint32_t pa[4]; // P rounded to the values' type; the row sums take the unrounded ones
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float sub = m[r] == -INFINITY ? 0.f : m[r];
+                    float e[4];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x)
+                            e[h * 2 + x] = ex2_approx(fmaf(sc[h][2 * r + x], p.sl2, -sub));
+                    l[r] = l[r] * alpha[r] + ((e[0] + e[1]) + (e[2] + e[3]));
+                    pa[r] = pack2<F16>(e[0], e[1]), pa[2 + r] = pack2<F16>(e[2], e[3]);
+                }
+                if (__any_sync(0xffffffffu, need)) {
+#pragma unroll
+                    for (int i = 0; i < HD / 8; ++i)
+                        o[i][0] *= alpha[0], o[i][1] *= alpha[0], o[i][2] *= alpha[1], o[i][3] *= alpha[1];
+                }
+                // V's pairs of keys (2 quad, 2 quad + 1) and 8 on: which to keep in a block's last keys
+                uint32_t mask[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int key = h * 8 + quad * 2;
+                    mask[h] = (key < keys ? 0xffffu : 0u) | (key + 1 < keys ? 0xffff0000u : 0u);
+                }
+#pragma unroll
+                for (int i = 0; i < HD / 16; ++i) {
+                    const int piece = (i & 3) * 2 + v_piece;
+                    uint32_t b[4];
+                    ldmatrix4_trans(b, sv + (i >> 2) * (FEW_KEYS * 128) + v_row * 128 + ((piece ^ (v_row & 7)) << 4));
+                    mma16816<F16>(o[2 * i], pa, b[0] & mask[0], b[1] & mask[1]);
+                    mma16816<F16>(o[2 * i + 1], pa, b[2] & mask[0], b[3] & mask[1]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(&empty[s]);
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) { // a row's sum over its four threads
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        }
+    }
+    // The parts: (max, sum) and output of every warp's rows, over the ring.
+    __syncthreads();
+    float2* ml = reinterpret_cast<float2*>(smem + SM::OFF_ML);
+    float* out = reinterpret_cast<float*>(smem);
+    if (warp > 0) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int at = (warp - 1) * FEW_ROWS + row_a + 8 * r;
+            if (quad == 0)
+                ml[at] = ok ? make_float2(m[r], l[r]) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i)
+                *reinterpret_cast<float2*>(out + at * HD + i * 8 + quad * 2) = make_float2(o[i][2 * r], o[i][2 * r + 1]);
+        }
+    }
+    __syncthreads();
+    // A warp a row: lane z of `parts` (at most 16) has part z's (max, sum) and gets its weight; returns the rows' (max, sum).
+    auto weigh = [&](float2 a, float& w) {
+        float mx = a.x;
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1)
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+        w = a.y == 0.f ? 0.f : ex2_approx(a.x - (mx == -INFINITY ? 0.f : mx));
+        float sum = w * a.y;
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1)
+            sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        return make_float2(__shfl_sync(0xffffffffu, mx, 0), __shfl_sync(0xffffffffu, sum, 0));
+    };
+    const int piece = lane < HD / 4 ? lane : 0;
+    auto store = [&](int r, float4 v, float sum) {
+        int row, head;
+        if (!row_of(r, row, head) || lane >= HD / 4)
+            return;
+        const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum); // no key (or none above -infinity): 0; a NaN stays one
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + size_t(row) * p.out_stride + head * HD + piece * 4) =
+            make_uint2(pack2<F16>(v.x * inv, v.y * inv), pack2<F16>(v.z * inv, v.w * inv));
+    };
+    const int rows = min(run_rows, run.q1 - run.row0) * p.group;
+    for (int r = warp; r < rows; r += FEW_NT / 32) {
+        float w;
+        const float2 all = weigh(lane < FEW_WARPS ? ml[lane * FEW_ROWS + r] : make_float2(-INFINITY, 0.f), w);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int z = 0; z < FEW_WARPS; ++z) {
+            const float wz = __shfl_sync(0xffffffffu, w, z);
+            const float4 v = *reinterpret_cast<const float4*>(out + (z * FEW_ROWS + r) * HD + piece * 4);
+            if (wz != 0.f) // a part of no weight may hold anything
+                acc.x += wz * v.x, acc.y += wz * v.y, acc.z += wz * v.z, acc.w += wz * v.w;
+        }
+        if (split == 1) {
+            store(r, acc, all.y);
+        } else {
+            if (lane == 0)
+                ml[FEW_WARPS * FEW_ROWS + r] = all;
+            if (lane < HD / 4)
+                *reinterpret_cast<float4*>(out + (FEW_WARPS * FEW_ROWS + r) * HD + piece * 4) = acc;
+        }
+    }
+    if (split > 1) {
+        cluster_sync();
+        for (int r = int(part) + warp * int(split); r < rows; r += int(split) * (FEW_NT / 32)) {
+            float w;
+            const float2 all = weigh(lane < int(split) ? ld_cluster2(smem_u32(ml + FEW_WARPS * FEW_ROWS + r), lane) : make_float2(-INFINITY, 0.f), w);
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+            for (int z = 0; z < int(split); ++z) {
+                const float wz = __shfl_sync(0xffffffffu, w, z);
+                const float4 v = ld_cluster4(smem_u32(out + (FEW_WARPS * FEW_ROWS + r) * HD + piece * 4), z);
+                if (wz != 0.f)
+                    acc.x += wz * v.x, acc.y += wz * v.y, acc.z += wz * v.z, acc.w += wz * v.w;
+            }
+            store(r, acc, all.y);
+        }
+        cluster_sync(); // no CTA leaves while another reads its shared memory
+    }
+}
+
+// A run as this CTA has it: TWO query tiles, each of which sees every block of the CTA, or one, whose even blocks are "tile"
+// 0's and odd ones tile 1's.
+template <int HD, bool F16, bool TWO>
+__device__ __forceinline__ void attend(const PkMaps& maps, const PkArgs& p, const Run& run, int kv_head, uint32_t split, uint32_t part, int a_blocks,
+                                       int blocks)
 {
     using SM = PkSmem<HD>;
     constexpr int TL = SM::TL, OFF_K = SM::OFF_K, OFF_V = SM::OFF_V;
@@ -129,51 +498,30 @@ __global__ void __launch_bounds__(NT, 1) packed_attention_kernel(const __grid_co
     uint64_t* q_full = bars + 0;
     uint64_t* k_full = bars + 1;       // [KST]
     uint64_t* k_empty = k_full + KST;  // [KST]
-    uint64_t* v_full = k_empty + KST;  // [VST]
-    uint64_t* v_empty = v_full + VST;  // [VST]
-    uint64_t* s_full = v_empty + VST;  // [2] per tile
+    uint64_t* v_full = k_empty + KST;      // [VST + 1]
+    uint64_t* v_empty = v_full + VST + 1;  // [VST + 1]
+    uint64_t* s_full = v_empty + VST + 1;  // [2] per tile
     uint64_t* p_full = s_full + 2;     // [2] per tile
     uint64_t* pv_done = p_full + 2;    // [2] per tile
     uint64_t* drain = pv_done + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
 
-    const int warp = warp_id();
-    uint32_t split, part; // CTAs of this run's cluster, this one's number
-    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(split));
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(part));
-    const int slot = blockIdx.x / split, kv_head = blockIdx.y;
-    const int run = 4 * p.unit_rows;
-
-    if (blockIdx.x == 0 && blockIdx.y == 0) // the starts ascend within the tensors; a document with others is left out
-        for (int d = threadIdx.x; d <= p.docs; d += NT) {
-            const int a = p.q_start[d], b = p.k_start[d];
-            if (a < 0 || a > p.q_rows || b < 0 || b > p.k_rows || (d > 0 && (a < p.q_start[d - 1] || b < p.k_start[d - 1])))
-                record_error(kErrBadShape);
-        }
-
-    // This CTA's query rows [row0, q1) and the keys [0, a_end) and [b0, b_end) of their document.
-    const int doc = find_document(p, slot, run);
-    if (doc < 0)
-        return;
-    const int q0 = __ldg(p.q_start + doc), q1 = __ldg(p.q_start + doc + 1);
-    const int row0 = q0 + (slot - (q0 / run + doc)) * run;
-    int b0 = __ldg(p.k_start + doc), b_end = __ldg(p.k_start + doc + 1);
-    if (q0 < 0 || row0 < q0 || row0 >= q1 || q1 > p.q_rows || b0 < 0 || b_end < b0 || b_end > p.k_rows)
-        return;
-    int a_end = p.prefix;
-    b0 = max(b0, p.prefix);
-    b_end = max(b_end, b0);
-    if (b0 == p.prefix)
-        a_end = b_end, b0 = b_end; // the document's keys adjoin the prefix: one run
-    const int a_blocks = (a_end + 127) / 128;
-    const int blocks = a_blocks + (b_end - b0 + 127) / 128;
+    const int warp = __shfl_sync(0xffffffffu, warp_id(), 0);
+    const int row0 = run.row0, q1 = run.q1;
     const int per = (blocks + int(split) - 1) / int(split);
     const int first = min(int(part) * per, blocks);
     const int nkv = min(per, blocks - first); // this CTA's blocks [first, first + nkv)
     // first row and rows of this CTA's block j
-    auto block_row = [&](int j) { return first + j < a_blocks ? 128 * (first + j) : b0 + 128 * (first + j - a_blocks); };
-    auto block_keys = [&](int j) { return min(128, (first + j < a_blocks ? a_end : b_end) - block_row(j)); };
-    const bool two = row0 + 2 * p.unit_rows < q1; // the second tile has rows
+    auto block_row = [&](int j) { return first + j < a_blocks ? 128 * (first + j) : run.b0 + 128 * (first + j - a_blocks); };
+    auto block_keys = [&](int j) { return min(128, (first + j < a_blocks ? run.a_end : run.b_end) - block_row(j)); };
+    constexpr int vst = TWO ? VST : VST + 1;
+    // With so few blocks that joining two parts would take longer than it saves, tile 0 has them all.
+    const bool alternate = !TWO && (split > 1 || blocks >= 4);
+    auto steps = [&](int t) { return TWO ? nkv : alternate ? (nkv + 1 - t) >> 1 : t ? 0 : nkv; }; // of tile t
+    auto block_of = [&](int t, int i) { return alternate ? 2 * i + t : i; };                     // its i-th block
+    const bool join = split > 1 || alternate; // rows have several parts
+    auto k_slot = [&](int j) { return OFF_K + (j % KST) * TL; };
+    auto v_slot = [&](int j) { return j % vst < VST ? OFF_V + (j % vst) * TL : TL; };
 
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
@@ -181,7 +529,7 @@ __global__ void __launch_bounds__(NT, 1) packed_attention_kernel(const __grid_co
             mbar_init(&k_full[i], 1);
             mbar_init(&k_empty[i], 1);
         }
-        for (int i = 0; i < VST; ++i) {
+        for (int i = 0; i < VST + 1; ++i) {
             mbar_init(&v_full[i], 1);
             mbar_init(&v_empty[i], 1);
         }
@@ -204,8 +552,7 @@ __global__ void __launch_bounds__(NT, 1) packed_attention_kernel(const __grid_co
 
     if (warp == 0 && elect_one_lane()) {
         // ------------------------------------------------------------------------------------------ TMA
-        const int units = two ? 4 : 2;
-        bool ok = true;
+        const int units = TWO ? 4 : 2;
         if (nkv > 0) {
             mbar_arrive_expect_tx(q_full, uint32_t(units * p.unit_rows * p.group * HD * 2));
             for (int u = 0; u < units; ++u)
@@ -226,16 +573,14 @@ __global__ void __launch_bounds__(NT, 1) packed_attention_kernel(const __grid_co
         int jk = 0, jv = 0;
         while (jv < nkv) {
             if (jk < nkv && jk < jv + KST) {
-                const int s = jk % KST;
-                if (!(ok = mbar_wait(&k_empty[s], ((jk / KST) & 1) ^ 1)))
+                if (!mbar_wait(&k_empty[jk % KST], ((jk / KST) & 1) ^ 1))
                     break;
-                load(smem + OFF_K + s * TL, &maps.k, &k_full[s], jk);
+                load(smem + k_slot(jk), &maps.k, &k_full[jk % KST], jk);
                 ++jk;
             } else {
-                const int s = jv % VST;
-                if (!(ok = mbar_wait(&v_empty[s], ((jv / VST) & 1) ^ 1)))
+                if (!mbar_wait(&v_empty[jv % vst], ((jv / vst) & 1) ^ 1))
                     break;
-                load(smem + OFF_V + s * TL, &maps.v, &v_full[s], jv);
+                load(smem + v_slot(jv), &maps.v, &v_full[jv % vst], jv);
                 ++jv;
             }
         }
@@ -244,66 +589,67 @@ __global__ void __launch_bounds__(NT, 1) packed_attention_kernel(const __grid_co
             mbar_wait(q_full, 0);
         for (int j = max(0, jk - KST); j < jk; ++j)
             mbar_wait(&k_full[j % KST], (j / KST) & 1);
-        for (int j = max(0, jv - VST); j < jv; ++j)
-            mbar_wait(&v_full[j % VST], (j / VST) & 1);
-    } else if (warp == 1 && elect_one_lane()) {
+        for (int j = max(0, jv - vst); j < jv; ++j)
+            mbar_wait(&v_full[j % vst], (j / vst) & 1);
+    } else if (warp == 1) {
         // ------------------------------------------------------------------------------------------ MMA
+        // The warp stays converged and one lane issues, so that descriptors are made in uniform registers.
+        uint32_t elected;
+        asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
         const uint32_t id_s = idesc_16<F16>(128, 128, false);
         const uint32_t id_pv = idesc_16<F16>(128, HD, true);
-        auto issue_s = [&](int t, int j) {
-            const int ks = j % KST;
-            const uint32_t sq = smem_u32(smem + t * TL);
-            const uint32_t sk = smem_u32(smem + OFF_K + ks * TL);
-#pragma unroll
-            for (int kk = 0; kk < HD / 16; ++kk) {
-                const uint32_t off = (kk >> 2) * HALF + (kk & 3) * 32;
-                mma_bf16_ss(tmem + t * 128, sdesc_sw128(sq + off, 16, 1024), sdesc_sw128(sk + off, 16, 1024), id_s, kk > 0);
-            }
-            mma_commit(&s_full[t]);
-            if (t == 1 || !two)
-                mma_commit(&k_empty[ks]); // every tile's S MMAs have read K_j
-        };
-        auto issue_pv = [&](int t, int j) {
-            const int vs = j % VST;
-            const uint32_t sv = smem_u32(smem + OFF_V + vs * TL);
-#pragma unroll
-            for (int kk = 0; kk < 8; ++kk)
-                mma_bf16_ts(tmem + 256 + t * HD, tmem + t * 128 + kk * 8, sdesc_sw128(sv + kk * 2048, HALF, 1024), id_pv, (j | kk) != 0);
-            mma_commit(&pv_done[t]);
-            if (t == 1 || !two)
-                mma_commit(&v_empty[vs]); // every tile's PV MMAs have read V_j
-        };
-        bool ok = nkv > 0 && mbar_wait(q_full, 0) && mbar_wait(&k_full[0], 0);
-        if (ok) {
+        const uint32_t smem0 = smem_u32(smem);
+        // tile t's i-th scores, once their keys are there
+        auto scores = [&](int t, int i) {
+            const int j = block_of(t, i);
+            if (!mbar_wait(&k_full[j % KST], (j / KST) & 1))
+                return false;
             tc_fence_after();
-            issue_s(0, 0);
-            if (two)
-                issue_s(1, 0);
-        }
-        for (int j = 0; j < nkv && ok; ++j) {
-            if (!(ok = mbar_wait(&v_full[j % VST], (j / VST) & 1) && mbar_wait(&p_full[0], j & 1)))
-                break;
+            const uint64_t qd = sdesc_sw128(smem0 + (TWO ? t * TL : 0), 16, 1024), kd = sdesc_sw128(smem0 + k_slot(j), 16, 1024);
+            if (elected) {
+#pragma unroll
+                for (int kk = 0; kk < HD / 16; ++kk) {
+                    constexpr int half = HALF >> 4, piece = 32 >> 4;
+                    const int off = (kk >> 2) * half + (kk & 3) * piece;
+                    mma_bf16_ss(tmem + t * 128, qd + off, kd + off, id_s, kk > 0);
+                }
+                mma_commit(&s_full[t]);
+                if (t == 1 || !TWO)
+                    mma_commit(&k_empty[j % KST]); // every tile's S MMAs have read K_j
+            }
+            __syncwarp();
+            return true;
+        };
+        // its i-th product with V, once P is there
+        auto values = [&](int t, int i) {
+            const int j = block_of(t, i);
+            if (!mbar_wait(&v_full[j % vst], (j / vst) & 1) || !mbar_wait(&p_full[t], i & 1))
+                return false;
             tc_fence_after();
-            issue_pv(0, j);
-            const bool more = j + 1 < nkv;
-            if (more) {
-                if (!(ok = mbar_wait(&k_full[(j + 1) % KST], ((j + 1) / KST) & 1)))
-                    break;
-                tc_fence_after();
-                issue_s(0, j + 1);
+            const uint64_t vd = sdesc_sw128(smem0 + v_slot(j), HALF, 1024);
+            if (elected) {
+#pragma unroll
+                for (int kk = 0; kk < 8; ++kk)
+                    mma_bf16_ts(tmem + 256 + t * HD, tmem + t * 128 + kk * 8 + (kk >= 4 ? 32 : 0), vd + kk * (2048 >> 4), id_pv, i > 0 || kk > 0);
+                mma_commit(&pv_done[t]);
+                if (t == 1 || !TWO)
+                    mma_commit(&v_empty[j % vst]); // every tile's PV MMAs have read V_j
             }
-            if (two) {
-                if (!(ok = mbar_wait(&p_full[1], j & 1)))
-                    break;
-                tc_fence_after();
-                issue_pv(1, j);
-                if (more)
-                    issue_s(1, j + 1);
-            }
+            __syncwarp();
+            return true;
+        };
+        const int n0 = steps(0), n1 = steps(1);
+        bool ok = nkv > 0 && mbar_wait(q_full, 0) && scores(0, 0) && (n1 == 0 || scores(1, 0));
+        for (int i = 0; i < n0 && ok; ++i) {
+            ok = values(0, i) && (i + 1 >= n0 || scores(0, i + 1));
+            if (ok && i < n1)
+                ok = values(1, i) && (i + 1 >= n1 || scores(1, i + 1));
         }
-        mma_commit(drain);
+        if (elected)
+            mma_commit(drain);
+        __syncwarp();
         mbar_wait(drain, 0);
-    } else if (warp >= 2 && (two || warp < 6)) {
+    } else if (warp >= 2) {
         // -------------------------------------------------------------------------------------- softmax
         const int t = (warp - 2) / 4;
         const int quarter = warp & 3;
@@ -313,75 +659,65 @@ __global__ void __launch_bounds__(NT, 1) packed_attention_kernel(const __grid_co
         const uint32_t tO = tmem + lane_base + 256 + t * HD;
         // this thread's query row and head
         const int in_unit = row & 63;
-        const int out_row = row0 + (2 * t + (row >> 6)) * p.unit_rows + in_unit / p.group;
+        const int out_row = row0 + ((TWO ? 2 * t : 0) + (row >> 6)) * p.unit_rows + in_unit / p.group;
         const bool valid = in_unit < p.unit_rows * p.group && out_row < q1;
         const bool idle = !__any_sync(0xffffffffu, valid); // rows that nobody asked for: their P may be anything
         float m = -INFINITY, l = 0.f;
         bool ok = true;
-        for (int j = 0; j < nkv; ++j) {
-            if (!(ok = mbar_wait(&s_full[t], j & 1)))
+        const int n = steps(t);
+        for (int step = 0; step < n; ++step) {
+            if (!(ok = mbar_wait(&s_full[t], step & 1)))
                 break;
             tc_fence_after();
+            const int j = block_of(t, step);
             const int keys = block_keys(j);
-            if (t == 0 && keys < 128) {
-                // V rows past the block's keys
-                if (!(ok = mbar_wait(&v_full[j % VST], (j / VST) & 1)))
+            if (keys < 128 && (t == 0 || !TWO)) {
+                // V rows past the block's keys (two tiles: before tile 0's PV, which comes first)
+                if (!(ok = mbar_wait(&v_full[j % vst], (j / vst) & 1)))
                     break;
-                uint8_t* sv = smem + OFF_V + (j % VST) * TL;
-                for (int i = keys * 8 + row; i < 128 * 8; i += 128)
+                uint8_t* sv = smem + v_slot(j);
+                for (int c = keys * 8 + row; c < 128 * 8; c += 128)
 #pragma unroll
                     for (int hh = 0; hh < HD / 64; ++hh)
-                        *reinterpret_cast<uint4*>(sv + hh * HALF + i * 16) = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4*>(sv + hh * HALF + c * 16) = make_uint4(0, 0, 0, 0);
                 fence_proxy_async_smem();
             }
             if (!idle) {
-                float s[128];
-                {
-                    uint32_t r[4][32];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        tmem_ld32(tS + c * 32, r[c]);
+                // The scores in halves of 64 keys, so that no more than one is in registers: both for the maximum, then the
+                // second and the first (read again) for P, which is written over its own half.
+                float s[64];
+                auto half = [&](int h) {
+                    uint32_t r[2][32];
+                    tmem_ld32(tS + h * 64, r[0]);
+                    tmem_ld32(tS + h * 64 + 32, r[1]);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            s[c * 32 + i] = __uint_as_float(r[c][i]);
-                }
-                if (keys < 128) {
-#pragma unroll
-                    for (int c = 0; c < 128; ++c)
-                        if (c >= keys)
-                            s[c] = -INFINITY;
-                }
+                    for (int c = 0; c < 64; ++c)
+                        s[c] = __uint_as_float(r[c >> 5][c & 31]);
+                };
+                if (keys < 128)
+                    hide_columns(tS, keys);
                 float mp[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    mp[i] = fmaxf(s[2 * i], s[2 * i + 1]);
-#pragma unroll
-                for (int c = 16; c < 128; c += 16)
+                for (int h = 0; h < 2; ++h) {
+                    half(h);
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        mp[i] = max3f(mp[i], s[c + 2 * i], s[c + 2 * i + 1]);
+                        mp[i] = h ? max3f(mp[i], s[2 * i], s[2 * i + 1]) : fmaxf(s[2 * i], s[2 * i + 1]);
+#pragma unroll
+                    for (int c = 16; c < 64; c += 16)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            mp[i] = max3f(mp[i], s[c + 2 * i], s[c + 2 * i + 1]);
+                }
                 const float mx = max3f(max3f(mp[0], mp[1], mp[2]), max3f(mp[3], mp[4], mp[5]), fmaxf(mp[6], mp[7]));
                 const float m_cand = mx * p.sl2;
                 const bool need = m_cand > m + kRescaleThreshold;
                 const float m_use = need ? m_cand : m;
                 const float alpha = need ? ex2_approx(m - m_use) : 1.f;
                 const float msub = m_use == -INFINITY ? 0.f : m_use;
-                const float2 scale2 = make_float2(p.sl2, p.sl2), neg2 = make_float2(-msub, -msub);
-                float2 sp[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-                uint32_t pk[64]; // P rounded to the values' type for the tensor core; the row sum takes the unrounded ones
-#pragma unroll
-                for (int c = 0; c < 64; ++c) {
-                    const float2 x = fma2(make_float2(s[2 * c], s[2 * c + 1]), scale2, neg2);
-                    const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-                    sp[c & 3] = add2(sp[c & 3], e);
-                    pk[c] = pack2<F16>(e.x, e.y);
-                }
-                const float2 s01 = add2(add2(sp[0], sp[1]), add2(sp[2], sp[3]));
-                if (j > 0 && __any_sync(0xffffffffu, need)) {
-                    // O_t holds PV_t(0..j-1), complete (S_t(j) was issued after PV_t(j-1))
+                if (step > 0 && __any_sync(0xffffffffu, need)) {
+                    // O_t holds the PVs before, complete (these scores were issued after the last of them)
 #pragma unroll 1
                     for (int c = 0; c < HD / 32; ++c) {
                         uint32_t o[32];
@@ -393,11 +729,25 @@ __global__ void __launch_bounds__(NT, 1) packed_attention_kernel(const __grid_co
                         tmem_st32(tO + c * 32, o);
                     }
                 }
+                const float2 scale2 = make_float2(p.sl2, p.sl2), neg2 = make_float2(-msub, -msub);
+                float2 sp[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                for (int h = 1; h >= 0; --h) {
+                    if (h == 0)
+                        half(0);
+                    uint32_t pk[32]; // P rounded to the values' type for the tensor core; the row sum takes the unrounded ones
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) {
+                        const float2 x = fma2(make_float2(s[2 * c], s[2 * c + 1]), scale2, neg2);
+                        const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                        sp[c & 3] = add2(sp[c & 3], e);
+                        pk[c] = pack2<F16>(e.x, e.y);
+                    }
+                    tmem_st32(tS + h * 64, pk);
+                }
+                const float2 s01 = add2(add2(sp[0], sp[1]), add2(sp[2], sp[3]));
                 l = l * alpha + (s01.x + s01.y);
                 m = m_use;
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-                    tmem_st32(tS + c * 32, *reinterpret_cast<uint32_t(*)[32]>(pk + c * 32));
                 tmem_wait_st();
             }
             tc_fence_before();
@@ -405,39 +755,40 @@ __global__ void __launch_bounds__(NT, 1) packed_attention_kernel(const __grid_co
             if (elect_one_lane())
                 mbar_arrive(&p_full[t]);
         }
-        const bool done = ok && (nkv == 0 || mbar_wait(&pv_done[t], (nkv - 1) & 1));
-        tc_fence_after();
-        if (split > 1) {
-            // This part's unnormalised rows and their (max, sum), for the join below. A part that gave up counts for
-            // nothing (the device error says so); one without keys too.
-            const bool have = done && nkv > 0;
-            float2* ml = reinterpret_cast<float2*>(smem) + t * 128 + row;
+        const bool done = ok && (n == 0 || mbar_wait(&pv_done[t], (n - 1) & 1));
+        if (join) {
+            // This part's unnormalised rows and their (max, sum), for the join below, over Q and the rings: the other
+            // tile's MMAs must be done with them too. A part that gave up counts for nothing (the device error says so),
+            // as one without keys.
+            const int other = steps(t ^ 1);
+            const bool all = done && (other == 0 || mbar_wait(&pv_done[t ^ 1], (other - 1) & 1)) && n > 0;
+            tc_fence_after();
             float* o_row = reinterpret_cast<float*>(smem + OFF_K) + size_t(t * 128 + row) * HD;
-            // Q and the rings are read by MMAs that are complete for this tile only: wait for the other one too
-            const bool all = have && (!two || mbar_wait(&pv_done[t ^ 1], (nkv - 1) & 1));
             if (!idle) {
-                *ml = all ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+                reinterpret_cast<float2*>(smem)[t * 128 + row] = all ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
                 if (all) {
 #pragma unroll 1
                     for (int c = 0; c < HD / 32; ++c) {
                         uint32_t o[32];
                         tmem_ld32(tO + c * 32, o);
                         tmem_wait_ld();
+                        if (valid)
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) // 16-byte pieces swizzled over the banks
-                            *reinterpret_cast<float4*>(o_row + (((c * 8 + i) ^ (row & 7)) << 2)) =
-                                make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
-                                            __uint_as_float(o[4 * i + 3]));
+                            for (int i = 0; i < 8; ++i) // 16-byte pieces swizzled over the banks
+                                *reinterpret_cast<float4*>(o_row + (((c * 8 + i) ^ (row & 7)) << 2)) =
+                                    make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
+                                                __uint_as_float(o[4 * i + 3]));
                     }
                 }
             }
-        } else if (done && !idle) {
+        } else if (done && !idle && (TWO || t == 0)) {
+            tc_fence_after();
             const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l); // no key (or none above -infinity): 0; a NaN stays one
             uint16_t* dst = static_cast<uint16_t*>(p.out) + size_t(out_row) * p.out_stride + (kv_head * p.group + in_unit % p.group) * HD;
 #pragma unroll 1
             for (int c = 0; c < HD / 32; ++c) {
                 uint32_t o[32];
-                if (nkv > 0) {
+                if (n > 0) {
                     tmem_ld32(tO + c * 32, o);
                     tmem_wait_ld();
                 } else {
@@ -464,31 +815,38 @@ __global__ void __launch_bounds__(NT, 1) packed_attention_kernel(const __grid_co
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
-    if (split > 1) {
-        // Join: a warp a row, the rows dealt out over the cluster's CTAs; parts weighted by 2^(m_part - max), in their order.
-        cluster_sync();
-        const int rows = two ? 256 : 128;
+    if (join) {
+        // A warp a row, the rows dealt out over the cluster's CTAs; parts weighted by 2^(m_part - max), in their order.
+        if (split > 1)
+            cluster_sync();
+        const int rows = TWO ? 256 : 128, tiles = TWO ? 1 : 2; // tiles: parts of a row in a CTA
         for (int r = int(part) + warp * int(split); r < rows; r += int(split) * (NT / 32)) {
             const int in_unit = r & 63;
             const int out_row = row0 + (r >> 6) * p.unit_rows + in_unit / p.group;
             if (in_unit >= p.unit_rows * p.group || out_row >= q1)
                 continue;
-            const uint32_t ml = smem_u32(smem) + r * 8;
-            float mx = -INFINITY;
-            for (uint32_t z = 0; z < split; ++z)
-                mx = fmaxf(mx, ld_cluster2(ml, z).x);
-            const float sub = mx == -INFINITY ? 0.f : mx;
+            const int parts = int(split) * tiles;
+            // lane z holds part z's (max, sum): CTA z / tiles, tile z % tiles
+            float2 a = make_float2(-INFINITY, 0.f);
+            if (lane_id() < parts)
+                a = ld_cluster2(smem_u32(smem) + (lane_id() % tiles * 128 + r) * 8, lane_id() / tiles);
+            float mx = a.x;
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1)
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o, 16));
+            mx = __shfl_sync(0xffffffffu, mx, 0);
+            const float w_part = a.y == 0.f ? 0.f : ex2_approx(a.x - (mx == -INFINITY ? 0.f : mx));
             float sum = 0.f;
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
             const int piece = lane_id() < HD / 4 ? lane_id() : 0;
-            const uint32_t o = smem_u32(smem + OFF_K) + r * HD * 4 + ((piece ^ (r & 7)) << 4);
-            for (uint32_t z = 0; z < split; ++z) {
-                const float2 a = ld_cluster2(ml, z);
-                if (a.y == 0.f)
+#pragma unroll 4
+            for (int z = 0; z < parts; ++z) {
+                const float w = __shfl_sync(0xffffffffu, w_part, z), l = __shfl_sync(0xffffffffu, a.y, z);
+                if (l == 0.f)
                     continue; // a part without keys has written no row
-                const float w = ex2_approx(a.x - sub);
-                const float4 v = ld_cluster4(o, z);
-                sum += w * a.y;
+                const int at = z % tiles * 128 + r;
+                const float4 v = ld_cluster4(smem_u32(smem + OFF_K) + at * HD * 4 + ((piece ^ (at & 7)) << 4), z / tiles);
+                sum += w * l;
                 acc.x += w * v.x, acc.y += w * v.y, acc.z += w * v.z, acc.w += w * v.w;
             }
             const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
@@ -497,8 +855,30 @@ __global__ void __launch_bounds__(NT, 1) packed_attention_kernel(const __grid_co
                 *reinterpret_cast<uint2*>(dst + piece * 4) = make_uint2(pack2<F16>(acc.x * inv, acc.y * inv), pack2<F16>(acc.z * inv, acc.w * inv));
             }
         }
-        cluster_sync(); // no CTA leaves while another reads its shared memory
+        if (split > 1)
+            cluster_sync(); // no CTA leaves while another reads its shared memory
     }
+}
+
+template <int HD, bool F16>
+__global__ void __launch_bounds__(NT, 1) packed_attention_kernel(const __grid_constant__ PkMaps maps, const PkArgs p)
+{
+    uint32_t split, part; // CTAs of this run's cluster, this one's number
+    cluster_place(split, part);
+    if (blockIdx.x == 0 && blockIdx.y == 0)
+        check_starts(p, NT);
+    const Run run = run_of(p, blockIdx.x / split, 4 * p.unit_rows);
+    if (!run.any)
+        return;
+    const int a_blocks = (run.a_end + 127) / 128;
+    const int blocks = a_blocks + (run.b_end - run.b0 + 127) / 128;
+    split = parts_of(blocks, LEAST, split);
+    if (part >= split)
+        return; // (a cluster barrier waits for the threads that are left)
+    if (run.row0 + 2 * p.unit_rows < run.q1)
+        attend<HD, F16, true>(maps, p, run, blockIdx.y, split, part, a_blocks, blocks);
+    else
+        attend<HD, F16, false>(maps, p, run, blockIdx.y, split, part, a_blocks, blocks);
 }
 
 CUtensorMap rows_map(const void* base, bool f16, int heads, int rows, int64_t stride, int head_dim, int box_heads, int box_rows)
@@ -510,20 +890,51 @@ CUtensorMap rows_map(const void* base, bool f16, int heads, int rows, int64_t st
 }
 
 template <int HD, bool F16>
-void launch(const PkMaps& maps, const PkArgs& a, int slots, int kv_heads, int split, cudaStream_t s)
+void launch(const PackedAttnParams& p, const PkMaps& maps, const PkArgs& a, cudaStream_t s)
 {
-    static std::atomic<uint64_t> opt_in;
-    smem_opt_in(packed_attention_kernel<HD, F16>, PkSmem<HD>::TOTAL, opt_in);
     cudaLaunchConfig_t c{};
-    c.gridDim = dim3(unsigned(slots) * split, kv_heads);
-    c.blockDim = dim3(NT);
-    c.dynamicSmemBytes = PkSmem<HD>::TOTAL;
-    c.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = unsigned(split), at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     c.attrs = at;
     c.numAttrs = 1;
+    c.stream = s;
+    // Every run of every document has a slot: q_start[d] / rows + d is a document's first, and the last is under this.
+    auto grid = [&](int rows, int split) {
+        at[0].val.clusterDim.x = unsigned(split);
+        c.gridDim = dim3(unsigned((long long)(p.q_rows / rows + p.docs) * split), p.kv_heads);
+    };
+    const long long keys = p.prefix + (p.k_rows - p.prefix) / p.docs; // an average document's
+    // The CTAs of a run's cluster: doubled while there are at most `room` in all and an average document would use half of
+    // them (`least` keys each); a run without the keys for all of them leaves some out.
+    auto split_of = [&](int rows, int room, int least, int most) {
+        const long long runs = std::max<long long>(p.docs, (p.q_rows + rows - 1) / rows) * p.kv_heads;
+        int split = 1;
+        while (split < most && runs * split * 2 <= room && keys >= (long long)split * least)
+            split *= 2;
+        return split;
+    };
+    // Documents of a few rows on average (two runs of 16 stacked rows at most) go to the kernel for few rows.
+    if (a.group <= FEW_ROWS && (long long)p.q_rows * a.group <= 2LL * FEW_ROWS * p.docs) {
+        static std::atomic<uint64_t> opt_in, wide;
+        smem_opt_in(few_rows_kernel<HD, F16>, FewSmem<HD>::TOTAL, opt_in);
+        if (!(wide.load() & device_bit())) {
+            H3_CUDA(cudaFuncSetAttribute(few_rows_kernel<HD, F16>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+            wide.fetch_or(device_bit());
+        }
+        const int rows = FEW_ROWS / a.group;
+        grid(rows, split_of(rows, 4 * num_sms(), FEW_LEAST * FEW_KEYS, FEW_SPLIT));
+        c.blockDim = dim3(FEW_NT);
+        c.dynamicSmemBytes = FewSmem<HD>::TOTAL;
+        H3_CUDA(cudaLaunchKernelEx(&c, few_rows_kernel<HD, F16>, maps, a, p.q, p.q_stride));
+        return;
+    }
+    static std::atomic<uint64_t> opt_in;
+    smem_opt_in(packed_attention_kernel<HD, F16>, PkSmem<HD>::TOTAL, opt_in);
+    const int rows = 4 * a.unit_rows;
+    grid(rows, split_of(rows, num_sms(), LEAST * 128, 8));
+    c.blockDim = dim3(NT);
+    c.dynamicSmemBytes = PkSmem<HD>::TOTAL;
     H3_CUDA(cudaLaunchKernelEx(&c, packed_attention_kernel<HD, F16>, maps, a));
 }
 
@@ -531,7 +942,7 @@ void launch(const PkMaps& maps, const PkArgs& a, int slots, int kv_heads, int sp
 
 void attention_packed(const PackedAttnParams& p, cudaStream_t s)
 {
-    const int group = p.heads / p.kv_heads, unit_rows = 64 / group, run = 4 * unit_rows;
+    const int group = p.heads / p.kv_heads, unit_rows = 64 / group;
     PkMaps maps;
     maps.q = rows_map(p.q, p.f16, p.heads, p.q_rows, p.q_stride, p.head_dim, group, unit_rows);
     // without key rows there is nothing to describe, and no load is made
@@ -541,18 +952,10 @@ void attention_packed(const PackedAttnParams& p, cudaStream_t s)
     a.out = p.out, a.out_stride = p.out_stride, a.q_start = p.q_start, a.k_start = p.k_start, a.q_rows = p.q_rows, a.k_rows = p.k_rows;
     a.docs = p.docs, a.prefix = p.prefix, a.group = group, a.unit_rows = unit_rows;
     a.sl2 = float(double(p.scale) * 1.4426950408889634);
-    // Every run of every document has a slot: a / run + d is a document's first, and the last is at most this.
-    const int slots = p.q_rows / run + p.docs;
-    // Split the keys while the CTAs would still fit the SMs at once and each keeps four blocks of keys.
-    const long long runs = std::max<long long>(p.docs, (p.q_rows + run - 1) / run);
-    const long long blocks = (p.prefix + (p.k_rows - p.prefix) / p.docs + 127) / 128;
-    int split = 1;
-    while (split < 8 && runs * p.kv_heads * split * 2 <= num_sms() && blocks >= split * 8)
-        split *= 2;
     if (p.head_dim == 128)
-        (p.f16 ? launch<128, true> : launch<128, false>)(maps, a, slots, p.kv_heads, split, s);
+        (p.f16 ? launch<128, true> : launch<128, false>)(p, maps, a, s);
     else
-        (p.f16 ? launch<64, true> : launch<64, false>)(maps, a, slots, p.kv_heads, split, s);
+        (p.f16 ? launch<64, true> : launch<64, false>)(p, maps, a, s);
 }
 
 } // namespace h3
