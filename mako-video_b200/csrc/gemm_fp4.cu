@@ -3,21 +3,23 @@
 //
 // One CTA per SM: warp 0 loads (TMA tiles of 128 bytes = 256 values of K, 128-byte swizzled; the scale tiles by plain bulk
 // copies), warp 1 issues, warps 2..9 are the epilogue. Per stage the issuer copies the stage's scale tiles from shared
-// memory into TMEM (tcgen05.cp, in order before the MMAs that read them) and runs four M = 128, N = 256, K = 64 MMAs. The
-// issue itself is what a stage's 12 copies and 4 MMAs in 512 clocks strain: descriptors are made once a stage and the
-// warp stays converged (one lane chosen by elect.sync), which took 33024 x 15360 x 5120 without an epilogue from 1.68 ms
-// to 0.93.
+// memory into TMEM (tcgen05.cp, in order before the MMAs that read them) and runs four MMAs of K = 64 and 128 rows x 256
+// columns per SM. The issue itself is what a stage's 12 copies and 4 MMAs in 512 clocks strain: descriptors are made once a
+// stage and the warp stays converged (one lane chosen by elect.sync), which took 33024 x 15360 x 5120 without an epilogue
+// from 1.68 ms to 0.93.
 //
-// TMEM: two accumulators of 256 columns and the scales do not fit 512 columns side by side, and N = 256 is what keeps the
-// shared-memory reads of an MMA (12 KB) under its time, so the accumulators overlap in 96 columns:
-//   [0, 256) accumulator 0, [160, 416) accumulator 1, [416, 512) two buffers of one stage's scales (48 columns each)
-// The epilogue's eight warps take a finished accumulator into registers at once (128 columns a thread) and hand TMEM on;
-// the next tile's MMAs wait for that, not for the arithmetic and the stores. A scale buffer is written again only after
-// the MMAs that read it are known to be complete (the stage's `empty` barrier), two stages later: the stage between keeps
-// the tensor core busy meanwhile.
+// Three forms:
+//   pair   (more than 128 rows) the two CTAs of a cluster share a tile of 256 x 256: each loads its 128 rows of A and half of
+//          B's, the first CTA issues for both (cta_group::2). A stage is 38 KB instead of 54 and five fit, which matters
+//          because at 54 KB in 512 clocks an SM's share of the L2 bandwidth, not the tensor core, sets the pace.
+//   tiles  (at most 128 rows) a CTA walks tiles of 128 x 256
+//   split  (fewer such tiles than half the SMs) the K of a tile is split over the CTAs of a cluster; they leave their sums in
+//          shared memory and each finishes a share of the tile from all of them, in their order
 //
-// With fewer tiles than SMs (few rows), the K of a tile is split over the CTAs of a cluster instead of one CTA walking
-// tiles; they leave their sums in shared memory and each finishes a share of the tile from all of them, in their order.
+// TMEM: the accumulator's 256 columns, then the scales of every stage of the ring (48 columns each for nv), so that a stage's
+// `empty` barrier covers its scales too; a second accumulator would leave none of the 512 for them. The epilogue's eight
+// warps take a finished accumulator into registers at once (128 columns a thread), and the next tile's MMAs start while
+// they do the arithmetic and the stores.
 #include "common.hpp"
 #include "fp4.cuh"
 #include "gemm_tiles.cuh"
@@ -32,26 +34,34 @@ namespace {
 
 constexpr int BM = 128, BN = 256;
 constexpr int KSTAGE = 256;          // values of K per stage: 128 bytes of codes a row
-constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128;
+constexpr int A_BYTES = BM * 128;
 constexpr int EPI_WARPS = 8;
 constexpr int NUM_THREADS = 64 + 32 * EPI_WARPS;
-constexpr int STAGES = 3;
-constexpr int ACC1 = 160;            // accumulator 1's first column
-constexpr int SCALE_COL = 416, SCALE_BUF = 48;
-constexpr int MAX_SPLIT = 8;         // CTAs of a cluster
+constexpr int SCALE_COL = BN, SCALE_COLS = 48; // TMEM: the first stage's scales, columns a stage
+constexpr int MAX_SPLIT = 8;         // CTAs of a cluster that share a tile's K
 
-template <Fp4 F>
+enum class Form { tiles, split, pair };
+
+template <Fp4 F, Form W>
 struct Fp4Smem {
+    static constexpr int STAGES = W == Form::pair ? 5 : 3;
+    static constexpr int B_ROWS = W == Form::pair ? BN / 2 : BN; // of a tile, in this CTA
+    static constexpr int B_BYTES = B_ROWS * 128;
     // scale tiles of a stage: 4 (nv) or 2 (mx) along K for A's 128 rows and twice as many for B's 256
     static constexpr int KT = KSTAGE / (4 * fp4_block(F));
     static constexpr int SF_BYTES = 3 * KT * 512;
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SF_BYTES;
-    static constexpr int OFF_STAGING = STAGES * STAGE_BYTES;             // 4 KB an epilogue warp: 32 rows of 128 bytes
-    static constexpr int OFF_COLS = OFF_STAGING + EPI_WARPS * 4096;      // its columns' scales and biases, 2 x 128 floats
-    static constexpr int OFF_BAR = OFF_COLS + EPI_WARPS * 1024;
+    // 4 KB an epilogue warp: 32 rows of 128 bytes of output; before that its columns' scales and biases, 2 x 128 floats
+    static constexpr int OFF_STAGING = STAGES * STAGE_BYTES;
+    static constexpr int OFF_BAR = OFF_STAGING + EPI_WARPS * 4096;
     static constexpr int TOTAL = OFF_BAR + 256 + 1024;
-    static_assert(STAGE_BYTES % 1024 == 0 && TOTAL <= 227 * 1024);
+    static_assert(STAGE_BYTES % 1024 == 0 && TOTAL <= 227 * 1024 && BN + STAGES * 48 <= 512);
     static_assert(BM * BN * 4 <= OFF_STAGING); // a split tile's sums, over the ring
+};
+
+// A's and B's codes (byte of K, row), and their scale tiles (word of a tile, tile).
+struct Fp4Inputs {
+    CUtensorMap a, b, a_scales, b_scales;
 };
 
 // Destination of the tiles: q/k/v one map per rank that owns heads (dim, q/k/v x head slot, row), else m[0] (column, row).
@@ -61,49 +71,135 @@ struct Fp4Maps {
     CUtensorMap m[EPI == Epi::qkv ? 8 : 1];
 };
 
-// D[tmem] (+)= A[smem] B[smem]^T on e2m1 codes, the block scales in TMEM at sfa and sfb.
-template <Fp4 F>
+// D[tmem] (+)= A[smem] B[smem]^T on e2m1 codes, the block scales in TMEM at sfa and sfb. PAIR: on both CTAs of the pair, each
+// with its own rows of A and D, half of B's rows, its scales of A and all of B's.
+#define H3_MMA_FP4(GROUP, KIND)                                                                                                   \
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"                                                               \
+                 "tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),                 \
+                 "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)                                                   \
+                 : "memory")
+template <Fp4 F, bool PAIR>
 __device__ __forceinline__ void mma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate)
 {
-    if constexpr (F == Fp4::nv)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-                     "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-                     "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-                     : "memory");
+    if constexpr (F == Fp4::nv && PAIR)
+        H3_MMA_FP4("2", "mxf4nvf4.block_scale.scale_vec::4X");
+    else if constexpr (F == Fp4::nv)
+        H3_MMA_FP4("1", "mxf4nvf4.block_scale.scale_vec::4X");
+    else if constexpr (PAIR)
+        H3_MMA_FP4("2", "mxf4.block_scale.scale_vec::2X");
     else
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-                     "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-                     "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-                     : "memory");
+        H3_MMA_FP4("1", "mxf4.block_scale.scale_vec::2X");
 }
+#undef H3_MMA_FP4
 
 // Instruction descriptor of the two kinds: e2m1 A and B, both K-major; the scales' type (1: powers of two, 0: e4m3) and
 // which pair of the scale bytes of a TMEM word the MMA reads (mx: a word holds two MMAs' scales).
-template <Fp4 F>
+template <Fp4 F, bool PAIR>
 __device__ __forceinline__ constexpr uint32_t idesc_fp4(uint32_t pair)
 {
-    return (pair << 4) | (1u << 7) | (1u << 10) | (uint32_t(BN >> 3) << 17) | (uint32_t(F == Fp4::mx) << 23) | (uint32_t(BM >> 7) << 27) |
-           (pair << 29);
+    return (pair << 4) | (1u << 7) | (1u << 10) | (uint32_t(BN >> 3) << 17) | (uint32_t(F == Fp4::mx) << 23) |
+           (uint32_t((PAIR ? 2 * BM : BM) >> 7) << 27) | (pair << 29);
 }
 
 // The scale copies and MMAs of one stage: `tiles` scale tiles along K and `steps` MMAs (constants in full stages, so that
 // the loops unroll). Scale tile k of A goes to columns tsf + 12 k, of B's two row halves to the next four and four.
-template <Fp4 F>
+template <Fp4 F, bool PAIR>
 __device__ __forceinline__ void issue_stage(uint32_t d, uint64_t ad, uint64_t bd, uint64_t fd, uint32_t tsf, int tiles, int steps, bool fresh)
 {
-    constexpr int KT = Fp4Smem<F>::KT;
+    constexpr int KT = Fp4Smem<F, Form::tiles>::KT;
 #pragma unroll
     for (int k = 0; k < tiles; ++k)
 #pragma unroll
-        for (int x = 0; x < 3; ++x)
+        for (int x = 0; x < 3; ++x) {
             // one tile, 32 rows of 16 bytes, into four columns of 32 lanes, repeated for the four lane quarters
-            asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tsf + k * 12 + x * 4), "l"(fd + (x * KT + k) * (512 >> 4))
-                         : "memory");
+            const uint64_t from = fd + (x * KT + k) * (512 >> 4);
+            if constexpr (PAIR)
+                asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tsf + k * 12 + x * 4), "l"(from) : "memory");
+            else
+                asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tsf + k * 12 + x * 4), "l"(from) : "memory");
+        }
 #pragma unroll
     for (int k = 0; k < steps; ++k) {
         const uint32_t sf = tsf + (F == Fp4::nv ? k : k / 2) * 12;
-        mma_fp4<F>(d, ad + k * (32 >> 4), bd + k * (32 >> 4), idesc_fp4<F>(F == Fp4::nv ? 0 : (k & 1) * 2), sf, sf + 4, !fresh || k > 0);
+        mma_fp4<F, PAIR>(d, ad + k * (32 >> 4), bd + k * (32 >> 4), idesc_fp4<F, PAIR>(F == Fp4::nv ? 0 : (k & 1) * 2), sf, sf + 4, !fresh || k > 0);
     }
+}
+
+// Arrive on `bar` (of both CTAs of a pair) once every tcgen05 operation this thread issued before has completed.
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint64_t* bar)
+{
+    if constexpr (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+                     "h"(uint16_t(3))
+                     : "memory");
+    else
+        mma_commit(bar);
+}
+
+// Arrives on the barrier at the same place in CTA `rank` of the cluster. (What it orders is tensor memory, by the tcgen05
+// fences around it.)
+__device__ __forceinline__ void arrive_cluster(uint64_t* bar, uint32_t rank)
+{
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, %1;\n\tmbarrier.arrive.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_u32(bar)),
+                 "r"(rank)
+                 : "memory");
+}
+
+// A TMA tile into this CTA's shared memory that completes on `bar`, a shared::cluster address: a pair's first CTA counts the
+// loads of both.
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const void* tmap, uint32_t bar, int32_t c0, int32_t c1)
+{
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];" ::"r"(
+                     smem_u32(dst)),
+                 "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(c0), "r"(c1)
+                 : "memory");
+}
+
+// mbar_wait for a barrier that the cluster's other CTA arrives on.
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity)
+{
+    auto done = [&] {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, 1000000;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok)
+                     : "r"(smem_u32(bar)), "r"(parity)
+                     : "memory");
+        return ok != 0;
+    };
+    if (done())
+        return true;
+    const long long t0 = clock64();
+    for (uint32_t i = 1;; ++i) {
+        if (done())
+            return true;
+        if (clock64() - t0 > 4000000000ll) {
+            record_error(kErrWaitTimeout);
+            return false;
+        }
+        if ((i & 255) == 0 && *(volatile uint32_t*)&g_device_error != 0)
+            return false;
+    }
+}
+
+template <bool PAIR>
+__device__ __forceinline__ void tmem_get(uint32_t* slot)
+{
+    if constexpr (PAIR) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+        tmem_alloc(slot, 512);
+        tmem_relinquish();
+    }
+}
+template <bool PAIR>
+__device__ __forceinline__ void tmem_free(uint32_t tmem)
+{
+    if constexpr (PAIR)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    else
+        tmem_dealloc(tmem, 512);
 }
 
 __device__ __forceinline__ void tma_reduce_add_2d(const void* tmap, const void* smem_src, int32_t c0, int32_t c1)
@@ -149,11 +245,12 @@ __device__ __forceinline__ uint4 pack8(const float* v)
 
 // The epilogue of this warp's 32 rows x 128 columns: takes the accumulator (release() once it is in registers), then 4 KB
 // of finished output at a time through the warp's staging buffer, stored by TMA (which clips rows past M and columns past
-// N). cols: the columns' row scales of B, then their biases.
+// N). The buffer holds the columns' row scales of B and their biases first.
 template <Epi EPI, class Release>
-__device__ __forceinline__ void epilogue_fp4(const GemmParams& p, uint32_t taddr, int m0, int n0, int half, uint8_t* buf, const float* cols,
-                                             const Fp4Maps<EPI>& om, Release&& release)
+__device__ __forceinline__ void epilogue_fp4(const GemmParams& p, uint32_t taddr, int m0, int n0, int half, uint8_t* buf, const Fp4Maps<EPI>& om,
+                                             Release&& release)
 {
+    const float* cols = reinterpret_cast<const float*>(buf);
     const int gm = m0 + lane_id(); // m0: the warp's first row
     const bool valid = gm < p.M;
     const float a_scale = p.a_scale && valid ? __ldg(p.a_scale + gm) : 1.0f;
@@ -307,27 +404,27 @@ __device__ __forceinline__ void finish4(const GemmParams& p, float4 s, float4 u,
     }
 }
 
-// SPLIT: the CTAs of a cluster share one tile's K; else a CTA walks whole tiles.
-template <Epi EPI, Fp4 F, bool SPLIT>
+template <Epi EPI, Fp4 F, Form W>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
-    gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const uint8_t* a_scales,
-                    const uint8_t* b_scales, const GemmParams p, const __grid_constant__ Fp4Maps<EPI> om)
+    gemm_fp4_kernel(const __grid_constant__ Fp4Inputs in, const GemmParams p, const __grid_constant__ Fp4Maps<EPI> om)
 {
-    using SM = Fp4Smem<F>;
-    constexpr int KT = SM::KT;
+    using SM = Fp4Smem<F, W>;
+    constexpr int KT = SM::KT, STAGES = SM::STAGES;
+    constexpr bool SPLIT = W == Form::split, PAIR = W == Form::pair;
+    constexpr int TILE_M = PAIR ? 2 * BM : BM;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     uint8_t* smem = smem_raw + (((raw + 1023) & ~1023u) - raw);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SM::OFF_BAR);
-    uint64_t* full = bars;              // [STAGES]
+    uint64_t* full = bars;              // [STAGES] a stage has landed (pair: in both CTAs, counted in the first)
     uint64_t* empty = full + STAGES;    // [STAGES]
-    uint64_t* tfull = empty + STAGES;   // [2] an accumulator is complete
-    uint64_t* taken = tfull + 2;        // an accumulator is in the epilogue's registers
+    uint64_t* tfull = empty + STAGES;   // the accumulator is complete
+    uint64_t* taken = tfull + 1;        // it is in the epilogue's registers (pair: of both CTAs, in the first)
     uint64_t* drain = taken + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
 
     const int warp = __shfl_sync(0xffffffffu, warp_id(), 0);
-    const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN;
+    const int tiles_m = (p.M + TILE_M - 1) / TILE_M, tiles_n = (p.N + BN - 1) / BN;
     const int num_tiles = tiles_m * tiles_n;
     const int scale_tiles = fp4_scale_tiles(p.K, F);
     int first_tile = blockIdx.x, tile_step = gridDim.x;
@@ -340,24 +437,27 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         const int all = kb1; // every part has a stage: the launch has no more parts than stages
         kb0 = int(part) * all / int(split), kb1 = (int(part) + 1) * all / int(split);
     }
+    if constexpr (PAIR) {
+        asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(part));
+        first_tile = blockIdx.x / 2, tile_step = gridDim.x / 2;
+    }
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) {
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
         }
-        for (int i = 0; i < 2; ++i)
-            mbar_init(&tfull[i], 1);
-        mbar_init(taken, EPI_WARPS);
+        mbar_init(tfull, 1);
+        mbar_init(taken, PAIR ? 2 * EPI_WARPS : EPI_WARPS);
         mbar_init(drain, 1);
         fence_barrier_init();
     }
-    if (warp == 1) {
-        tmem_alloc(tmem_slot, 512);
-        tmem_relinquish();
-    }
+    if (warp == 1)
+        tmem_get<PAIR>(tmem_slot);
     tc_fence_before();
     __syncthreads();
+    if constexpr (PAIR)
+        cluster_sync(); // both CTAs' barriers and TMEM are there
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
@@ -368,29 +468,41 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
             int tm, tn;
             tile_coords(tile, tiles_m, tiles_n, tm, tn);
-            const bool second = tn * BN + 128 < p.N; // B's second 128 rows have scale tiles
+            const int m_tile = PAIR ? 2 * tm + int(part) : tm; // this CTA's 128 rows (past M in a pair's last tile: zeros)
             for (int kb = kb0; kb < kb1; ++kb, ++it) {
                 const int s = it % STAGES;
                 if (!(ok = mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1)))
                     break;
                 uint8_t* sa = smem + s * SM::STAGE_BYTES;
                 uint8_t* sb = sa + A_BYTES;
-                uint8_t* sf = sb + B_BYTES;
-                const uint32_t sf_bytes = uint32_t(min(KT, scale_tiles - kb * KT)) * 512;
-                mbar_arrive_expect_tx(&full[s], A_BYTES + B_BYTES + sf_bytes * (second ? 3 : 2));
-                tma_load_2d(sa, &tmA, &full[s], kb * 128, tm * BM);
-                tma_load_2d(sb, &tmB, &full[s], kb * 128, tn * BN);
-                bulk_load(sf, a_scales + (size_t(tm) * scale_tiles + kb * KT) * 512, sf_bytes, &full[s]);
-                bulk_load(sf + KT * 512, b_scales + (size_t(2 * tn) * scale_tiles + kb * KT) * 512, sf_bytes, &full[s]);
-                if (second)
-                    bulk_load(sf + 2 * KT * 512, b_scales + (size_t(2 * tn + 1) * scale_tiles + kb * KT) * 512, sf_bytes, &full[s]);
+                uint8_t* sf = sb + SM::B_BYTES;
+                const int b_row = tn * BN + (PAIR ? int(part) * SM::B_ROWS : 0);
+                if constexpr (PAIR) {
+                    // scale boxes are whole (a tile past the last one of a row range is the next range's, or zeros: not used)
+                    if (part == 0)
+                        mbar_arrive_expect_tx(&full[s], 2 * SM::STAGE_BYTES);
+                    uint32_t bar;
+                    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(bar) : "r"(smem_u32(&full[s])));
+                    tma_load_2d_pair(sa, &in.a, bar, kb * 128, m_tile * BM);
+                    tma_load_2d_pair(sb, &in.b, bar, kb * 128, b_row);
+                    tma_load_2d_pair(sf, &in.a_scales, bar, 0, m_tile * scale_tiles + kb * KT);
+                    tma_load_2d_pair(sf + KT * 512, &in.b_scales, bar, 0, 2 * tn * scale_tiles + kb * KT);
+                    tma_load_2d_pair(sf + 2 * KT * 512, &in.b_scales, bar, 0, (2 * tn + 1) * scale_tiles + kb * KT);
+                } else {
+                    mbar_arrive_expect_tx(&full[s], SM::STAGE_BYTES);
+                    tma_load_2d(sa, &in.a, &full[s], kb * 128, m_tile * BM);
+                    tma_load_2d(sb, &in.b, &full[s], kb * 128, b_row);
+                    tma_load_2d(sf, &in.a_scales, &full[s], 0, m_tile * scale_tiles + kb * KT);
+                    tma_load_2d(sf + KT * 512, &in.b_scales, &full[s], 0, 2 * tn * scale_tiles + kb * KT);
+                    tma_load_2d(sf + 2 * KT * 512, &in.b_scales, &full[s], 0, (2 * tn + 1) * scale_tiles + kb * KT);
+                }
             }
         }
         // Wait for the loads still in flight to land before the CTA can exit.
         if (ok)
             for (uint32_t j = it >= STAGES ? it - STAGES : 0; j < it; ++j)
                 mbar_wait(&empty[j % STAGES], (j / STAGES) & 1);
-    } else if (warp == 1) {
+    } else if (warp == 1 && (!PAIR || part == 0)) {
         // ------------------------------------------------------------------------------------- MMA issuer
         uint32_t elected;
         asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
@@ -398,42 +510,36 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         uint32_t it = 0, t_local = 0;
         bool ok = true;
         for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step, ++t_local) {
-            // the accumulator of the tile before, which shares columns with this one's, has been taken (and this one's own
-            // of two tiles ago before that)
-            if (t_local > 0 && !(ok = mbar_wait(taken, (t_local - 1) & 1)))
+            if (t_local > 0 && !(ok = mbar_wait_cluster(taken, (t_local - 1) & 1)))
                 break;
             tc_fence_after();
-            const uint32_t d = tmem + (t_local & 1) * ACC1;
             for (int kb = kb0; kb < kb1; ++kb, ++it) {
                 const int s = it % STAGES;
-                if (!(ok = mbar_wait(&full[s], (it / STAGES) & 1)))
-                    break;
-                // the MMAs of two stages ago, which read this scale buffer, are complete
-                if (it >= 2 && !(ok = mbar_wait(&empty[(it - 2) % STAGES], ((it - 2) / STAGES) & 1)))
+                if (!(ok = mbar_wait_cluster(&full[s], (it / STAGES) & 1)))
                     break;
                 tc_fence_after();
-                const uint32_t sa = smem0 + s * SM::STAGE_BYTES, sf = sa + A_BYTES + B_BYTES;
+                const uint32_t sa = smem0 + s * SM::STAGE_BYTES, sf = sa + A_BYTES + SM::B_BYTES;
                 const uint64_t ad = sdesc_sw128(sa, 16, 1024), bd = sdesc_sw128(sa + A_BYTES, 16, 1024);
                 // scale tiles: 8-row groups of 128 bytes, no swizzle
                 const uint64_t fd = uint64_t((sf >> 4) & 0x3FFF) | (uint64_t(128 >> 4) << 32) | (uint64_t(1) << 46);
-                const uint32_t tsf = tmem + SCALE_COL + (it & 1) * SCALE_BUF;
+                const uint32_t tsf = tmem + SCALE_COL + s * SCALE_COLS;
                 const int left = p.K - kb * KSTAGE;
                 if (elected) {
                     if (left >= KSTAGE)
-                        issue_stage<F>(d, ad, bd, fd, tsf, KT, KSTAGE / 64, kb == kb0);
+                        issue_stage<F, PAIR>(tmem, ad, bd, fd, tsf, KT, KSTAGE / 64, kb == kb0);
                     else
-                        issue_stage<F>(d, ad, bd, fd, tsf, scale_tiles - kb * KT, (left + 63) / 64, kb == kb0);
-                    mma_commit(&empty[s]);
+                        issue_stage<F, PAIR>(tmem, ad, bd, fd, tsf, scale_tiles - kb * KT, (left + 63) / 64, kb == kb0);
+                    commit<PAIR>(&empty[s]);
                 }
                 __syncwarp();
             }
             if (ok && elected)
-                mma_commit(&tfull[t_local & 1]);
+                commit<PAIR>(tfull);
             __syncwarp();
         }
         // Every MMA this warp issued has completed once `drain` flips.
         if (elected)
-            mma_commit(drain);
+            commit<PAIR>(drain);
         __syncwarp();
         mbar_wait(drain, 0);
     } else if (warp >= 2) {
@@ -446,7 +552,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             int tm, tn;
             tile_coords(first_tile, tiles_m, tiles_n, tm, tn);
             const int r = quarter * 32 + lane_id();
-            if (mbar_wait(&tfull[0], 0)) {
+            if (mbar_wait(tfull, 0)) {
                 tc_fence_after();
                 if (tm * BM + quarter * 32 < p.M) {
                     float4* row = reinterpret_cast<float4*>(smem) + r * (BN / 4);
@@ -465,31 +571,36 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             }
         } else {
             uint8_t* buf = smem + SM::OFF_STAGING + (warp - 2) * 4096;
-            float* cols = reinterpret_cast<float*>(smem + SM::OFF_COLS) + (warp - 2) * 256;
             auto release = [&] {
                 tc_fence_before();
                 __syncwarp();
-                if (elect_one_lane())
-                    mbar_arrive(taken);
+                if (elect_one_lane()) {
+                    if constexpr (PAIR)
+                        arrive_cluster(taken, 0);
+                    else
+                        mbar_arrive(taken);
+                }
             };
             uint32_t t_local = 0;
             for (int tile = first_tile; tile < num_tiles; tile += tile_step, ++t_local) {
-                const int acc = t_local & 1;
                 int tm, tn;
                 tile_coords(tile, tiles_m, tiles_n, tm, tn);
                 {
                     // the columns' scales and biases, four a lane, while the MMAs run
                     const int j = lane_id() * 4, col = tn * BN + chunk_col<EPI>(half, j >> 5) + (j & 31);
                     const float4 one = make_float4(1.f, 1.f, 1.f, 1.f), none = make_float4(0.f, 0.f, 0.f, 0.f);
+                    float* cols = reinterpret_cast<float*>(buf);
+                    if (lane_id() == 0)
+                        bulk_wait_read0(); // the tile before has been read from the buffer
+                    __syncwarp();
                     reinterpret_cast<float4*>(cols)[lane_id()] = p.b_scale && col < p.N ? __ldg(reinterpret_cast<const float4*>(p.b_scale + col)) : one;
                     reinterpret_cast<float4*>(cols + 128)[lane_id()] = p.bias && col < p.N ? __ldg(reinterpret_cast<const float4*>(p.bias + col)) : none;
                     __syncwarp();
                 }
-                if (!mbar_wait(&tfull[acc], (t_local >> 1) & 1))
+                if (!mbar_wait(tfull, t_local & 1))
                     break;
                 tc_fence_after();
-                epilogue_fp4<EPI>(p, tmem + lanes + acc * ACC1, tm * BM + quarter * 32, tn * BN, half, buf, cols, om, release);
-                __syncwarp(); // every lane has read `cols`
+                epilogue_fp4<EPI>(p, tmem + lanes, tm * TILE_M + (PAIR ? int(part) * BM : 0) + quarter * 32, tn * BN, half, buf, om, release);
             }
             if (lane_id() == 0)
                 bulk_wait0(); // the staged tiles' stores are complete
@@ -498,9 +609,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    if constexpr (PAIR)
+        cluster_sync(); // no MMA of the pair is under way
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem, 512);
+        tmem_free<PAIR>(tmem);
     }
     if constexpr (SPLIT) {
         // The tile's rows below M in groups of four columns (SwiGLU: of outputs), dealt out over the cluster's threads.
@@ -553,20 +666,26 @@ Fp4Maps<EPI> output_maps(const GemmParams& p)
     return om;
 }
 
-template <Epi EPI, Fp4 F, bool SPLIT>
+template <Epi EPI, Fp4 F, Form W>
 bool launch(const void* A, const void* a_scales, const void* B, const void* b_scales, const GemmParams& p, int tiles, int ctas, cudaStream_t s)
 {
-    using SM = Fp4Smem<F>;
+    using SM = Fp4Smem<F, W>;
     const uint64_t bytes = uint64_t(p.K) / 2;
     const uint64_t adims[2] = {bytes, uint64_t(p.M)}, bdims[2] = {bytes, uint64_t(p.N)}, pitch[1] = {bytes};
-    const uint32_t abox[2] = {128, BM}, bbox[2] = {128, BN};
-    const CUtensorMap ta = make_tmap(CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, A, adims, pitch, abox);
-    const CUtensorMap tb = make_tmap(CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, B, bdims, pitch, bbox);
+    const uint32_t abox[2] = {128, BM}, bbox[2] = {128, SM::B_ROWS};
+    Fp4Inputs in;
+    in.a = make_tmap(CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, A, adims, pitch, abox);
+    in.b = make_tmap(CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, B, bdims, pitch, bbox);
+    const uint64_t scale_tiles = fp4_scale_tiles(p.K, F), spitch[1] = {512};
+    const uint64_t asdims[2] = {128, (p.M + 127) / 128 * scale_tiles}, bsdims[2] = {128, (p.N + 127) / 128 * scale_tiles};
+    const uint32_t sbox[2] = {128, uint32_t(SM::KT)};
+    in.a_scales = make_tmap(CU_TENSOR_MAP_DATA_TYPE_INT32, 2, a_scales, asdims, spitch, sbox, false);
+    in.b_scales = make_tmap(CU_TENSOR_MAP_DATA_TYPE_INT32, 2, b_scales, bsdims, spitch, sbox, false);
     Fp4Maps<EPI> om{};
-    if constexpr (!SPLIT)
+    if constexpr (W != Form::split)
         om = output_maps<EPI>(p);
     static std::atomic<uint64_t> opt_in;
-    smem_opt_in(gemm_fp4_kernel<EPI, F, SPLIT>, SM::TOTAL, opt_in);
+    smem_opt_in(gemm_fp4_kernel<EPI, F, W>, SM::TOTAL, opt_in);
     cudaLaunchConfig_t c{};
     c.blockDim = dim3(NUM_THREADS);
     c.dynamicSmemBytes = SM::TOTAL;
@@ -575,13 +694,17 @@ bool launch(const void* A, const void* a_scales, const void* B, const void* b_sc
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     c.attrs = at;
-    int split = 1;
-    if constexpr (SPLIT) {
+    if constexpr (W == Form::pair) {
+        c.numAttrs = 1;
+        at[0].val.clusterDim.x = 2;
+    }
+    if constexpr (W == Form::split) {
+        int split;
         // the largest cluster of which the device holds one per tile at once, with a stage for every CTA
         c.numAttrs = 1;
         static ClusterLimits limits;
         for (split = std::min({ctas / tiles, MAX_SPLIT, (p.K + KSTAGE - 1) / KSTAGE}); split > 1; --split)
-            if (limits.at_once(gemm_fp4_kernel<EPI, F, true>, c, split) >= tiles)
+            if (limits.at_once(gemm_fp4_kernel<EPI, F, W>, c, split) >= tiles)
                 break;
         if (split < 2)
             return false;
@@ -589,20 +712,24 @@ bool launch(const void* A, const void* a_scales, const void* B, const void* b_sc
         ctas = tiles * split;
     }
     c.gridDim = dim3(unsigned(ctas));
-    H3_CUDA(cudaLaunchKernelEx(&c, gemm_fp4_kernel<EPI, F, SPLIT>, ta, tb, static_cast<const uint8_t*>(a_scales),
-                               static_cast<const uint8_t*>(b_scales), p, om));
+    H3_CUDA(cudaLaunchKernelEx(&c, gemm_fp4_kernel<EPI, F, W>, in, p, om));
     return true;
 }
 
 template <Epi EPI, Fp4 F>
 void run(const void* A, const void* a_scales, const void* B, const void* b_scales, const GemmParams& p, cudaStream_t s)
 {
-    const long long tiles = (long long)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
+    const long long tiles_n = (p.N + BN - 1) / BN, tiles = (p.M + BM - 1) / BM * tiles_n;
     const int sms = num_sms();
     if constexpr (EPI != Epi::qkv) // its norm runs along whole rows of a tile
-        if (tiles * 2 <= sms && p.K > KSTAGE && launch<EPI, F, true>(A, a_scales, B, b_scales, p, int(tiles), sms, s))
+        if (tiles * 2 <= sms && p.K > KSTAGE && launch<EPI, F, Form::split>(A, a_scales, B, b_scales, p, int(tiles), sms, s))
             return;
-    launch<EPI, F, false>(A, a_scales, B, b_scales, p, int(tiles), int(std::min<long long>(tiles, sms)), s);
+    if (p.M > BM) {
+        const long long pairs = (p.M + 2 * BM - 1) / (2 * BM) * tiles_n;
+        launch<EPI, F, Form::pair>(A, a_scales, B, b_scales, p, int(pairs), int(std::min<long long>(pairs, sms / 2)) * 2, s);
+    } else {
+        launch<EPI, F, Form::tiles>(A, a_scales, B, b_scales, p, int(tiles), int(std::min<long long>(tiles, sms)), s);
+    }
 }
 
 } // namespace
