@@ -2,16 +2,42 @@
 //
 // Both are bound by HBM: the quantiser reads a row once and keeps it in registers while the row's maximum is found (nv
 // has a scale a row), the inverse reads half a byte and writes two or four for each value. A thread takes runs of 16
-// values: an nv block, or half of an mx block whose two threads exchange their maxima by a shuffle.
+// values: an nv block, or half of an mx block whose two threads exchange their maxima by a shuffle. A run moves as one or
+// two 32-byte accesses where rows are so aligned (a 16-byte access at a 32-byte stride costs the L2 twice the requests).
 #include "common.hpp"
 #include "fp4.cuh"
 #include "ptx.cuh"
 
+#include <algorithm>
 #include <cuda_fp16.h>
 
 namespace h3 {
 
 namespace {
+
+// 32-byte accesses (32-byte aligned).
+__device__ __forceinline__ void load32(uint32_t* w, const void* p)
+{
+    asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "l"(p));
+}
+__device__ __forceinline__ void store32(void* p, const uint32_t* w)
+{
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+                 "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+        "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
 
 // Sixteen consecutive values of a row, as loaded.
 template <Elem T>
@@ -19,13 +45,19 @@ struct Run {
     static constexpr int WORDS = T == Elem::f32 ? 16 : 8;
     uint32_t w[WORDS];
 
-    __device__ __forceinline__ void load(const void* row, int c)
+    __device__ __forceinline__ void load(const void* row, int c, bool wide)
     {
-        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(row) + size_t(c) * (T == Elem::f32 ? 4 : 2));
+        const uint8_t* p = static_cast<const uint8_t*>(row) + size_t(c) * (T == Elem::f32 ? 4 : 2);
+        if (wide) {
 #pragma unroll
-        for (int i = 0; i < WORDS / 4; ++i) {
-            const uint4 v = __ldg(p + i);
-            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+            for (int i = 0; i < WORDS; i += 8)
+                load32(w + i, p + i * 4);
+        } else {
+#pragma unroll
+            for (int i = 0; i < WORDS; i += 4) {
+                const uint4 v = __ldg(reinterpret_cast<const uint4*>(p + i * 4));
+                w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+            }
         }
     }
     // The bits of the largest magnitude as fp32 (an infinity or a NaN is larger than every number, a NaN than an
@@ -85,6 +117,14 @@ __device__ __forceinline__ float from_e4m3(uint32_t b)
     return __half2float(__ushort_as_half(static_cast<unsigned short>(h & 0xffffu)));
 }
 
+// 1 / c rounded to nearest for the 126 positive e4m3 numbers: the approximate reciprocal (within an ulp) and a Newton step.
+__device__ __forceinline__ float reciprocal_e4m3(float c)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(c));
+    return fmaf(r, fmaf(-c, r, 1.f), r);
+}
+
 __device__ __forceinline__ float power_of_two(int e) // -127 <= e <= 127 (2^-127 is subnormal)
 {
     return __uint_as_float(e > -127 ? uint32_t(e + 127) << 23 : 0x00400000u);
@@ -104,24 +144,24 @@ __device__ __forceinline__ uint2 encode(const Run<T>& x, uint32_t most, float rg
         // 2^e with e = floor(log2 most) - 2: the division by it is exact, so the codes are those of the exact quotient
         const int e = max(int(most >> 23) - 127 - 2, -127);
         byte = uint32_t(e + 127);
-        const float inv = power_of_two(-e);
+        const float2 inv = make_float2(power_of_two(-e), power_of_two(-e));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float2 v = x.pair(i);
-            q[i] = make_float2(v.x * inv, v.y * inv);
-        }
+        for (int i = 0; i < 8; ++i)
+            q[i] = mul2(x.pair(i), inv);
     } else {
-        byte = to_e4m3(__fdiv_rn(__uint_as_float(most) * rg, 6.f));
+        // A quotient rounded to nearest from the divisor's rounded reciprocal: one residual step (Markstein). For the six here,
+        // and for the codes: x / c has to be exact where it lies on the border of two codes, where ties go by the code.
+        const float m = __uint_as_float(most) * rg;
+        const float m6 = m * (1.f / 6.f);
+        byte = to_e4m3(fmaf(fmaf(-m6, 6.f, m), 1.f / 6.f, m6));
         const float c = from_e4m3(byte);
-        const float inv = c > 0.f ? __frcp_rn(c) : 0.f;
-        // x / c rounded to nearest from the reciprocal (one residual step: exact where c has four bits), so that a quotient
-        // on the border of two codes is seen as one
+        const float inv = c > 0.f ? reciprocal_e4m3(c) : 0.f;
+        const float2 rg2 = make_float2(rg, rg), inv2 = make_float2(inv, inv), nc2 = make_float2(-c, -c);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float2 v = x.pair(i);
-            const float sx = v.x * rg, sy = v.y * rg;
-            const float qx = sx * inv, qy = sy * inv;
-            q[i] = make_float2(fmaf(fmaf(-qx, c, sx), inv, qx), fmaf(fmaf(-qy, c, sy), inv, qy));
+            const float2 s = mul2(x.pair(i), rg2);
+            const float2 f = mul2(s, inv2);
+            q[i] = fma2(fma2(f, nc2, s), inv2, f);
         }
     }
     return make_uint2(e2m1x8(q[0], q[1], q[2], q[3]), e2m1x8(q[4], q[5], q[6], q[7]));
@@ -132,19 +172,20 @@ __device__ __forceinline__ size_t scale_at(int row, int block, int tiles)
     return (size_t(row >> 7) * tiles + (block >> 2)) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
 }
 
-constexpr int QUANT_THREADS = 256;
-constexpr int QUANT_RUNS = 4; // runs of 16 values that a thread keeps
+constexpr int QUANT_RUNS = 2;    // runs of 16 values that a thread keeps: few, so that many threads have loads under way
+constexpr int QUANT_THREADS = 512; // of a CTA at most
 
-// WARPS warps a row, QUANT_THREADS / 32 / WARPS rows a CTA. A row of more than WARPS x 32 x RUNS runs (only with eight
-// warps) is read twice instead of kept.
-template <Elem T, Fp4 F, int WARPS, int RUNS>
-__global__ void __launch_bounds__(QUANT_THREADS) quant_fp4_kernel(const void* x, int64_t ldx, int rows, int K, uint8_t* codes, uint8_t* scales,
-                                                                  float* row_scale)
+// blockDim.x = 32 x the warps of a row (RUNS runs a thread; a row of more runs than that is read twice instead of kept), or,
+// for SHORT rows of one warp, of as many rows.
+// (64 registers a thread: 33024 x 5120 in 86 us for nv and 68 for mx; unbounded, with 72, 98 and 70.)
+template <Elem T, Fp4 F, bool SHORT>
+__global__ void __launch_bounds__(QUANT_THREADS, 2) quant_fp4_kernel(const void* x, int64_t ldx, int rows, int K, bool wide, uint8_t* codes,
+                                                                  uint8_t* scales, float* row_scale)
 {
-    constexpr int ROWS = QUANT_THREADS / 32 / WARPS, STEP = WARPS * 32;
+    constexpr int RUNS = QUANT_RUNS;
     __shared__ uint32_t red[QUANT_THREADS / 32];
-    const int r = blockIdx.x * ROWS + warp_id() / WARPS;
-    const int t = threadIdx.x % STEP;
+    const int r = SHORT ? blockIdx.x * (blockDim.x / 32) + warp_id() : blockIdx.x;
+    const int step = SHORT ? 32 : blockDim.x, t = SHORT ? lane_id() : threadIdx.x;
     const int runs = K / 16, tiles = fp4_scale_tiles(K, F);
     const bool in = r < rows;
     const uint8_t* row = static_cast<const uint8_t*>(x) + (in ? size_t(r) * ldx * (T == Elem::f32 ? 4 : 2) : 0);
@@ -155,36 +196,34 @@ __global__ void __launch_bounds__(QUANT_THREADS) quant_fp4_kernel(const void* x,
 #pragma unroll
     for (int i = 0; i < RUNS; ++i) {
         most[i] = 0;
-        if (in && t + i * STEP < runs)
-            keep[i].load(row, (t + i * STEP) * 16);
+        if (in && t + i * step < runs)
+            keep[i].load(row, (t + i * step) * 16, wide);
     }
 #pragma unroll
     for (int i = 0; i < RUNS; ++i)
-        if (in && t + i * STEP < runs) {
+        if (in && t + i * step < runs) {
             most[i] = keep[i].largest();
             all = max(all, most[i]);
         }
     float rg = 1.f;
     if constexpr (F == Fp4::nv) {
         if (in)
-            for (int c = t + RUNS * STEP; c < runs; c += STEP) {
+            for (int c = t + RUNS * step; c < runs; c += step) {
                 Run<T> a;
-                a.load(row, c * 16);
+                a.load(row, c * 16, wide);
                 all = max(all, a.largest());
             }
         all = __reduce_max_sync(0xffffffffu, all);
-        if constexpr (WARPS > 1) {
+        if constexpr (!SHORT) {
             if (lane_id() == 0)
                 red[warp_id()] = all;
             __syncthreads();
-#pragma unroll
-            for (int i = 0; i < WARPS; ++i)
-                all = max(all, red[warp_id() / WARPS * WARPS + i]);
+            all = __reduce_max_sync(0xffffffffu, lane_id() < int(blockDim.x) / 32 ? red[lane_id()] : 0);
         }
         // 2^(floor(log2 max) - 10): block scales up to 2^11 / 6 = 341.3, under e4m3's 448
         const int e = max(int(all >> 23) - 127 - 10, -126);
         const bool number = all < 0x7f800000u;
-        rg = number ? power_of_two(-e) : 0.f; // 0 x infinity is a NaN, whose code is replaced below
+        rg = number ? power_of_two(-e) : 0.f;
         if (in && t == 0)
             row_scale[r] = number ? power_of_two(e) : __uint_as_float(0x7fffffffu);
     }
@@ -213,14 +252,14 @@ __global__ void __launch_bounds__(QUANT_THREADS) quant_fp4_kernel(const void* x,
     };
 #pragma unroll
     for (int i = 0; i < RUNS; ++i)
-        if (i * STEP < padded) // the same for the whole CTA: the shuffles see full warps
-            finish(t + i * STEP, keep[i], most[i]);
-    for (int c0 = RUNS * STEP; c0 < padded; c0 += STEP) {
+        if (i * step < padded) // the same for the whole CTA: the shuffles see full warps
+            finish(t + i * step, keep[i], most[i]);
+    for (int c0 = RUNS * step; c0 < padded; c0 += step) {
         const int c = c0 + t;
         Run<T> a;
         uint32_t m = 0;
         if (in && c < runs) {
-            a.load(row, c * 16);
+            a.load(row, c * 16, wide);
             m = a.largest();
         }
         finish(c, a, m);
@@ -230,7 +269,7 @@ __global__ void __launch_bounds__(QUANT_THREADS) quant_fp4_kernel(const void* x,
 // A thread an output run of 16 values.
 template <Elem T, Fp4 F>
 __global__ void __launch_bounds__(256) dequant_fp4_kernel(const uint8_t* codes, const uint8_t* scales, const float* row_scale, int rows, int K,
-                                                          void* out, int64_t ldo)
+                                                          bool wide, void* out, int64_t ldo)
 {
     const int runs = K / 16, tiles = fp4_scale_tiles(K, F);
     const size_t id = size_t(blockIdx.x) * 256 + threadIdx.x;
@@ -255,47 +294,50 @@ __global__ void __launch_bounds__(256) dequant_fp4_kernel(const uint8_t* codes, 
         // code x block scale is exact (2 and 4 bits), so the product with the row's scale is the one rounding in fp32
         v[2 * i] = f.x * scale * g, v[2 * i + 1] = f.y * scale * g;
     }
-    if constexpr (T == Elem::f32) {
-        float4* d = reinterpret_cast<float4*>(static_cast<float*>(out) + size_t(r) * ldo + size_t(c) * 16);
+    constexpr int WORDS = Run<T>::WORDS;
+    uint32_t w[WORDS];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            d[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-    } else {
-        uint32_t w[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if constexpr (T == Elem::bf16) {
-                w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
-            } else {
-                const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-                w[i] = *reinterpret_cast<const uint32_t*>(&h);
-            }
+    for (int i = 0; i < 8; ++i) {
+        if constexpr (T == Elem::f32) {
+            w[2 * i] = __float_as_uint(v[2 * i]), w[2 * i + 1] = __float_as_uint(v[2 * i + 1]);
+        } else if constexpr (T == Elem::bf16) {
+            w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+        } else {
+            const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
         }
-        uint4* d = reinterpret_cast<uint4*>(static_cast<uint8_t*>(out) + (size_t(r) * ldo + size_t(c) * 16) * 2);
-        d[0] = make_uint4(w[0], w[1], w[2], w[3]);
-        d[1] = make_uint4(w[4], w[5], w[6], w[7]);
     }
+    uint8_t* d = static_cast<uint8_t*>(out) + (size_t(r) * ldo + size_t(c) * 16) * (T == Elem::f32 ? 4 : 2);
+    if (wide) {
+#pragma unroll
+        for (int i = 0; i < WORDS; i += 8)
+            store32(d + i * 4, w + i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < WORDS; i += 4)
+            *reinterpret_cast<uint4*>(d + i * 4) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+    }
+}
+
+// Whether every row starts on a 32-byte boundary.
+bool rows_wide(const void* p, int64_t ld, int rows, int size)
+{
+    return reinterpret_cast<uintptr_t>(p) % 32 == 0 && (rows == 1 || ld * size % 32 == 0);
 }
 
 template <Elem T, Fp4 F>
 void quant(const void* x, int64_t ldx, int rows, int K, void* codes, void* scales, float* row_scale, cudaStream_t s)
 {
     const int runs = K / 16, all_rows = (rows + 127) / 128 * 128;
-    auto launch = [&](auto kernel, int warps) {
-        const int per = QUANT_THREADS / 32 / warps;
-        kernel<<<(all_rows + per - 1) / per, QUANT_THREADS, 0, s>>>(x, ldx, rows, K, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales),
-                                                                    row_scale);
-        H3_CUDA(cudaGetLastError());
-    };
-    // the fewest warps a row that keep it in QUANT_RUNS runs a thread
-    if (runs <= 32 * QUANT_RUNS)
-        launch(quant_fp4_kernel<T, F, 1, QUANT_RUNS>, 1);
-    else if (runs <= 64 * QUANT_RUNS)
-        launch(quant_fp4_kernel<T, F, 2, QUANT_RUNS>, 2);
-    else if (runs <= 128 * QUANT_RUNS)
-        launch(quant_fp4_kernel<T, F, 4, QUANT_RUNS>, 4);
+    const bool wide = rows_wide(x, ldx, rows, T == Elem::f32 ? 4 : 2);
+    auto* c = static_cast<uint8_t*>(codes);
+    auto* sc = static_cast<uint8_t*>(scales);
+    const int warps = (runs + 32 * QUANT_RUNS - 1) / (32 * QUANT_RUNS);
+    if (warps == 1) // eight rows a CTA
+        quant_fp4_kernel<T, F, true><<<all_rows / 8, 256, 0, s>>>(x, ldx, rows, K, wide, c, sc, row_scale);
     else
-        launch(quant_fp4_kernel<T, F, 8, QUANT_RUNS>, 8);
+        quant_fp4_kernel<T, F, false><<<all_rows, std::min(32 * warps, QUANT_THREADS), 0, s>>>(x, ldx, rows, K, wide, c, sc, row_scale);
+    H3_CUDA(cudaGetLastError());
 }
 
 template <Elem T, Fp4 F>
@@ -303,7 +345,7 @@ void dequant(const void* codes, const void* scales, const float* row_scale, int 
 {
     const size_t n = size_t(rows) * (K / 16);
     dequant_fp4_kernel<T, F><<<unsigned((n + 255) / 256), 256, 0, s>>>(static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales),
-                                                                       row_scale, rows, K, out, ldo);
+                                                                       row_scale, rows, K, rows_wide(out, ldo, rows, T == Elem::f32 ? 4 : 2), out, ldo);
     H3_CUDA(cudaGetLastError());
 }
 
