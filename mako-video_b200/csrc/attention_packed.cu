@@ -190,14 +190,20 @@ __device__ __forceinline__ uint32_t parts_of(int blocks, int least, uint32_t mos
 }
 
 // ------------------------------------------------------------------------------------------------------------
-// Few rows: 16 / group query rows of a document (16 stacked rows), where the keys' bytes are what counts. A 128-row tile of
-// the tensor core would be nearly empty and, at 1400 clocks for 128 keys, slower than HBM; the warp-wide m16n8k16 MMA fits
-// the rows. Warp 0 streams 64-key blocks of K and V through a ring (TMA); warps 1..4 take 16 keys of each block, with a
-// maximum, a sum and an output of their own (no exchange until the end). Two CTAs an SM.
-//   S (16 x 16) = Q K^T: Q's fragments in registers, K's by ldmatrix; P stays in registers (an MMA's sums are the next one's
-//   A fragment); O (16 x HD) += P V, V's fragments by ldmatrix.trans. Keys past a block's end get -infinity and V 0.
-// The warps' and then the cluster's parts are joined in a fixed order.
+// Small runs, on the warp-wide m16n8k16 MMA. Warp 0 streams 64-key blocks of K and V through a ring (TMA); warps 1..4 have 16
+// stacked rows each, with a maximum, a sum and an output of their own:
+//   BY_KEYS  few rows (16 / group query rows a run), where the keys' bytes are what counts: a 128-row tile of the tensor core
+//            would be nearly empty and, at 1400 clocks for 128 keys, slower than HBM. The warps have the same rows and take
+//            16 keys of each block; their parts, and then the cluster's, are joined in a fixed order.
+//   by rows  short documents: 64 / group query rows a run, the warps' rows are different ones. A CTA is a fraction of the big
+//            kernel's, starts faster, and several fit an SM.
+// S (16 x 16 keys) = Q K^T: Q's fragments in registers, K's by ldmatrix; P stays in registers (an MMA's sums are the next
+// one's A fragment); O (16 x HD) += P V, V's fragments by ldmatrix.trans. Keys past a block's end get -infinity and V 0.
 constexpr int FEW_ROWS = 16, FEW_KEYS = 64, FEW_STAGES = 3, FEW_WARPS = 4, FEW_NT = 32 + 32 * FEW_WARPS, FEW_SPLIT = 16;
+// Stacked rows of an average document up to which heads of 64 dims go by rows: 24 documents and 6 heads take 4.6 against 7.7 us
+// at 16 rows, 8.5 against 12.3 at 64, 17.5 against 19.7 at 128 and 29.0 against 24.8 at 192 (behind a prefix of 512 keys 15.5
+// against 26.9 at 16, 38.5 against 36.1 at 128). Heads of 128 dims, four times the work a run, are faster in the big kernel.
+constexpr int SHORT_ROWS = 128;
 constexpr int FEW_LEAST = 16; // blocks that a CTA takes before another one joins it: about 8 us against 7 of starting and joining
 
 template <int HD>
@@ -234,8 +240,8 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <int HD, bool F16>
-__global__ void __launch_bounds__(FEW_NT, 2) few_rows_kernel(const __grid_constant__ PkMaps maps, const PkArgs p, const void* q, int64_t q_stride)
+template <int HD, bool F16, bool BY_KEYS>
+__global__ void __launch_bounds__(FEW_NT, 2) small_runs_kernel(const __grid_constant__ PkMaps maps, const PkArgs p, const void* q, int64_t q_stride)
 {
     using SM = FewSmem<HD>;
     constexpr int TL = SM::TL;
@@ -248,7 +254,9 @@ __global__ void __launch_bounds__(FEW_NT, 2) few_rows_kernel(const __grid_consta
     const int warp = warp_id(), lane = lane_id();
     uint32_t split, part;
     cluster_place(split, part);
-    const int kv_head = blockIdx.y, run_rows = FEW_ROWS / p.group;
+    constexpr int STACK = BY_KEYS ? FEW_ROWS : FEW_ROWS * FEW_WARPS; // stacked rows of a run
+    constexpr int SLICES = BY_KEYS ? 1 : FEW_KEYS / 16;              // 16-key slices of a block that a warp takes
+    const int kv_head = blockIdx.y, run_rows = STACK / p.group;
     if (blockIdx.x == 0 && blockIdx.y == 0)
         check_starts(p, FEW_NT);
     const Run run = run_of(p, blockIdx.x / split, run_rows);
@@ -256,7 +264,7 @@ __global__ void __launch_bounds__(FEW_NT, 2) few_rows_kernel(const __grid_consta
         return;
     const int a_blocks = (run.a_end + FEW_KEYS - 1) / FEW_KEYS;
     const int blocks = a_blocks + (run.b_end - run.b0 + FEW_KEYS - 1) / FEW_KEYS;
-    split = parts_of(blocks, FEW_LEAST, split);
+    split = BY_KEYS ? parts_of(blocks, FEW_LEAST, split) : 1;
     if (part >= split)
         return; // (a cluster barrier waits for the threads that are left)
     const int per = (blocks + int(split) - 1) / int(split);
@@ -273,7 +281,8 @@ __global__ void __launch_bounds__(FEW_NT, 2) few_rows_kernel(const __grid_consta
     }
     __syncthreads();
 
-    const int row_a = lane >> 2, quad = lane & 3; // this thread's stacked rows row_a and row_a + 8, its pair of columns
+    const int row_a = (BY_KEYS || warp == 0 ? 0 : (warp - 1) * FEW_ROWS) + (lane >> 2); // this thread's stacked rows: and row_a + 8
+    const int quad = lane & 3;                                                           // its pair of columns
     // the query row and head of stacked row r; false: none
     auto row_of = [&](int r, int& row, int& head) {
         row = run.row0 + r / p.group, head = kv_head * p.group + r % p.group;
@@ -320,7 +329,10 @@ __global__ void __launch_bounds__(FEW_NT, 2) few_rows_kernel(const __grid_consta
                 qf[k][1] = qb ? __ldg(qb + k * 8 + quad) : 0, qf[k][3] = qb ? __ldg(qb + k * 8 + 4 + quad) : 0;
             }
         }
-        const int key0 = (warp - 1) * 16; // this warp's keys of a block
+        const int key0 = BY_KEYS ? (warp - 1) * 16 : 0; // this warp's first key of a block
+        bool idle = false;                              // no row of this warp's is anybody's
+        if constexpr (!BY_KEYS)
+            idle = row_a - (lane >> 2) >= min(run_rows, run.q1 - run.row0) * p.group;
         // ldmatrix addresses: lane i gives row i % 8 of matrix i / 8. K: matrices (keys 0-7, 8 dims), (keys 0-7, next 8), (keys 8-15,
         // ...), ...; V: (keys 0-7, 8 dims), (keys 8-15, the same), (keys 0-7, next 8), ...
         const int k_row = key0 + (lane >> 4) * 8 + (lane & 7), k_piece = (lane >> 3) & 1;
@@ -329,70 +341,82 @@ __global__ void __launch_bounds__(FEW_NT, 2) few_rows_kernel(const __grid_consta
             const int s = j % FEW_STAGES;
             if (!(ok = mbar_wait(&full[s], (j / FEW_STAGES) & 1)))
                 break;
-            const int keys = (first + j < a_blocks ? run.a_end : run.b_end) - block_row(j) - key0; // this warp's keys, if under 16
-            if (keys > 0) {
+            const int keys = (first + j < a_blocks ? run.a_end : run.b_end) - block_row(j) - key0; // this warp's keys, if under its 16 or 64
+            if (keys > 0 && !idle) {
                 const uint32_t sk = smem_u32(smem + s * 2 * TL), sv = sk + TL;
-                float c[2][2][4] = {}; // [k half][key half]: two chains a sum
+                float sc[SLICES][2][4];
 #pragma unroll
-                for (int k = 0; k < HD / 16; ++k) {
-                    const int piece = (k & 3) * 2 + k_piece;
-                    uint32_t b[4];
-                    ldmatrix4(b, sk + (k >> 2) * (FEW_KEYS * 128) + k_row * 128 + ((piece ^ (k_row & 7)) << 4));
-                    mma16816<F16>(c[k & 1][0], qf[k], b[0], b[1]);
-                    mma16816<F16>(c[k & 1][1], qf[k], b[2], b[3]);
-                }
-                float sc[2][4];
+                for (int u = 0; u < SLICES; ++u) {
+                    float c[2][2][4] = {}; // [k half][key half]: two chains a sum
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int key = h * 8 + quad * 2 + (e & 1);
-                        sc[h][e] = key < keys ? c[0][h][e] + c[1][h][e] : -INFINITY;
+                    for (int k = 0; k < HD / 16; ++k) {
+                        const int piece = (k & 3) * 2 + k_piece;
+                        uint32_t b[4];
+                        ldmatrix4(b, sk + (k >> 2) * (FEW_KEYS * 128) + (u * 16 + k_row) * 128 + ((piece ^ (k_row & 7)) << 4));
+                        mma16816<F16>(c[k & 1][0], qf[k], b[0], b[1]);
+                        mma16816<F16>(c[k & 1][1], qf[k], b[2], b[3]);
                     }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int key = u * 16 + h * 8 + quad * 2 + (e & 1);
+                            sc[u][h][e] = key < keys ? c[0][h][e] + c[1][h][e] : -INFINITY;
+                        }
+                }
                 float alpha[2];
                 bool need = false;
 #pragma unroll
                 for (int r = 0; r < 2; ++r) { // rows row_a, row_a + 8
-                    float mx = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int u = 0; u < SLICES; ++u)
+                        mx = fmaxf(mx, fmaxf(fmaxf(sc[u][0][2 * r], sc[u][0][2 * r + 1]), fmaxf(sc[u][1][2 * r], sc[u][1][2 * r + 1])));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * p.sl2;
                     const bool grow = mx > m[r] + kRescaleThreshold;
                     alpha[r] = grow ? ex2_approx(m[r] - mx) : 1.f;
                     m[r] = grow ? mx : m[r];
+                    l[r] *= alpha[r];
                     need |= grow;
-                }
-                uint32_t pa[4]; // P rounded to the values' type; the row sums take the unrounded ones
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const float sub = m[r] == -INFINITY ? 0.f : m[r];
-                    float e[4];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int x = 0; x < 2; ++x)
-                            e[h * 2 + x] = ex2_approx(fmaf(sc[h][2 * r + x], p.sl2, -sub));
-                    l[r] = l[r] * alpha[r] + ((e[0] + e[1]) + (e[2] + e[3]));
-                    pa[r] = pack2<F16>(e[0], e[1]), pa[2 + r] = pack2<F16>(e[2], e[3]);
                 }
                 if (__any_sync(0xffffffffu, need)) {
 #pragma unroll
                     for (int i = 0; i < HD / 8; ++i)
                         o[i][0] *= alpha[0], o[i][1] *= alpha[0], o[i][2] *= alpha[1], o[i][3] *= alpha[1];
                 }
-                // V's pairs of keys (2 quad, 2 quad + 1) and 8 on: which to keep in a block's last keys
-                uint32_t mask[2];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int key = h * 8 + quad * 2;
-                    mask[h] = (key < keys ? 0xffffu : 0u) | (key + 1 < keys ? 0xffff0000u : 0u);
-                }
+                for (int u = 0; u < SLICES; ++u) {
+                    if (u * 16 >= keys)
+                        break;
+                    uint32_t pa[4]; // P rounded to the values' type; the row sums take the unrounded ones
 #pragma unroll
-                for (int i = 0; i < HD / 16; ++i) {
-                    const int piece = (i & 3) * 2 + v_piece;
-                    uint32_t b[4];
-                    ldmatrix4_trans(b, sv + (i >> 2) * (FEW_KEYS * 128) + v_row * 128 + ((piece ^ (v_row & 7)) << 4));
-                    mma16816<F16>(o[2 * i], pa, b[0] & mask[0], b[1] & mask[1]);
-                    mma16816<F16>(o[2 * i + 1], pa, b[2] & mask[0], b[3] & mask[1]);
+                    for (int r = 0; r < 2; ++r) {
+                        const float sub = m[r] == -INFINITY ? 0.f : m[r];
+                        float e[4];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int x = 0; x < 2; ++x)
+                                e[h * 2 + x] = ex2_approx(fmaf(sc[u][h][2 * r + x], p.sl2, -sub));
+                        l[r] += (e[0] + e[1]) + (e[2] + e[3]);
+                        pa[r] = pack2<F16>(e[0], e[1]), pa[2 + r] = pack2<F16>(e[2], e[3]);
+                    }
+                    // V's pairs of keys (2 quad, 2 quad + 1) and 8 on: which to keep in a block's last keys
+                    uint32_t mask[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int key = u * 16 + h * 8 + quad * 2;
+                        mask[h] = (key < keys ? 0xffffu : 0u) | (key + 1 < keys ? 0xffff0000u : 0u);
+                    }
+#pragma unroll
+                    for (int i = 0; i < HD / 16; ++i) {
+                        const int piece = (i & 3) * 2 + v_piece;
+                        uint32_t b[4];
+                        ldmatrix4_trans(b, sv + (i >> 2) * (FEW_KEYS * 128) + (u * 16 + v_row) * 128 + ((piece ^ (v_row & 7)) << 4));
+                        mma16816<F16>(o[2 * i], pa, b[0] & mask[0], b[1] & mask[1]);
+                        mma16816<F16>(o[2 * i + 1], pa, b[2] & mask[0], b[3] & mask[1]);
+                    }
                 }
             }
             __syncwarp();
@@ -404,6 +428,21 @@ __global__ void __launch_bounds__(FEW_NT, 2) few_rows_kernel(const __grid_consta
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
         }
+    }
+    if constexpr (!BY_KEYS) {
+        if (warp > 0 && ok)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                int row, head;
+                if (!row_of(row_a + 8 * r, row, head))
+                    continue;
+                const float inv = l[r] > 0.f ? 1.f / l[r] : (l[r] == 0.f ? 0.f : l[r]); // as in `store` below
+                uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + size_t(row) * p.out_stride + head * HD) + quad;
+#pragma unroll
+                for (int i = 0; i < HD / 8; ++i)
+                    dst[i * 4] = pack2<F16>(o[i][2 * r] * inv, o[i][2 * r + 1] * inv);
+            }
+        return;
     }
     // The parts: (max, sum) and output of every warp's rows, over the ring.
     __syncthreads();
@@ -914,21 +953,32 @@ void launch(const PackedAttnParams& p, const PkMaps& maps, const PkArgs& a, cuda
             split *= 2;
         return split;
     };
-    // Documents of a few rows on average (two runs of 16 stacked rows at most) go to the kernel for few rows.
-    if (a.group <= FEW_ROWS && (long long)p.q_rows * a.group <= 2LL * FEW_ROWS * p.docs) {
+    // Documents of a few rows on average (two runs of 16 stacked rows at most), and short ones, go to the kernel for small runs.
+    const long long stacked = (long long)p.q_rows * a.group;
+    if (a.group <= FEW_ROWS && stacked <= 2LL * FEW_ROWS * p.docs) {
         static std::atomic<uint64_t> opt_in, wide;
-        smem_opt_in(few_rows_kernel<HD, F16>, FewSmem<HD>::TOTAL, opt_in);
+        smem_opt_in(small_runs_kernel<HD, F16, true>, FewSmem<HD>::TOTAL, opt_in);
         if (!(wide.load() & device_bit())) {
-            H3_CUDA(cudaFuncSetAttribute(few_rows_kernel<HD, F16>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+            H3_CUDA(cudaFuncSetAttribute(small_runs_kernel<HD, F16, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
             wide.fetch_or(device_bit());
         }
         const int rows = FEW_ROWS / a.group;
         grid(rows, split_of(rows, 4 * num_sms(), FEW_LEAST * FEW_KEYS, FEW_SPLIT));
         c.blockDim = dim3(FEW_NT);
         c.dynamicSmemBytes = FewSmem<HD>::TOTAL;
-        H3_CUDA(cudaLaunchKernelEx(&c, few_rows_kernel<HD, F16>, maps, a, p.q, p.q_stride));
+        H3_CUDA(cudaLaunchKernelEx(&c, small_runs_kernel<HD, F16, true>, maps, a, p.q, p.q_stride));
         return;
     }
+    if constexpr (HD == 64)
+        if (stacked <= (long long)SHORT_ROWS * p.docs) {
+            static std::atomic<uint64_t> opt_in;
+            smem_opt_in(small_runs_kernel<HD, F16, false>, FewSmem<HD>::TOTAL, opt_in);
+            grid(FEW_ROWS * FEW_WARPS / a.group, 1);
+            c.blockDim = dim3(FEW_NT);
+            c.dynamicSmemBytes = FewSmem<HD>::TOTAL;
+            H3_CUDA(cudaLaunchKernelEx(&c, small_runs_kernel<HD, F16, false>, maps, a, p.q, p.q_stride));
+            return;
+        }
     static std::atomic<uint64_t> opt_in;
     smem_opt_in(packed_attention_kernel<HD, F16>, PkSmem<HD>::TOTAL, opt_in);
     const int rows = 4 * a.unit_rows;
