@@ -5,8 +5,9 @@
 // O in TMEM, P written back over S and read from there by the PV MMA; O rescaled only when a row's maximum grows by more
 // than 2^8. What differs:
 //   - A CTA is a run of query rows of one document. Launches have a slot for every run that the documents could need
-//     (a document of rows [a, b) owns the slots from a / TR + d on, TR rows a run), so the host needs no lengths; a slot
-//     without rows ends at once.
+//     (rows / TR + documents, TR rows a run), so the host needs no lengths; a slot without rows ends at once. Up to 32
+//     documents get their slots in the order of their keys, longest first, which leaves short runs for the end of a
+//     launch; of more, document d owns the slots from q_start[d] / TR + d on.
 //   - The `group` query heads of a kv head are stacked into the tile's rows (row r of the tile: query row r / group, head
 //     r % group, by the TMA box alone), so shared keys are loaded once for all of them, and one query row of a large
 //     group fills a tile.
@@ -57,7 +58,7 @@ struct PkArgs {
     int64_t out_stride;
     const int32_t* q_start;
     const int32_t* k_start;
-    int q_rows, k_rows, docs, prefix, group, unit_rows; // unit_rows: query rows in a 64-row unit, 64 / group
+    int q_rows, k_rows, kv_heads, docs, prefix, group, unit_rows; // unit_rows: query rows in a 64-row unit, 64 / group
     float sl2;                                          // scale log2(e)
 };
 
@@ -117,24 +118,44 @@ __device__ __forceinline__ float2 ld_cluster2(uint32_t addr, uint32_t rank)
 }
 
 struct Document {
-    int index, q0, q1, k0, k1;
+    int index, tile; // the document (-1: none), and which of its runs
+    int q0, q1, k0, k1;
 };
 
-// The document whose slots hold `slot`: the last d with q_start[d] / run + d <= slot (index -1: none). One warp, 32
-// candidates a step; the last step has read the starts by the time it knows which it needs.
+// The document and run of a slot. One warp: up to 32 documents a lane each, else 32 candidates a step for the last d with
+// q_start[d] / run + d <= slot; the last step has read the starts by the time it knows which it needs.
 __device__ __forceinline__ Document find_document(const PkArgs& p, int slot, int run)
 {
+    const int lane = lane_id();
     int lo = 0, n = p.docs;
     while (true) {
         const int step = (n + 31) / 32;
-        const bool in = lane_id() * step < n;
-        const int d = lo + (in ? lane_id() * step : 0);
+        const bool in = lane * step < n;
+        const int d = lo + (in ? lane * step : 0);
         const int q0 = __ldg(p.q_start + d), q1 = __ldg(p.q_start + d + 1), k0 = __ldg(p.k_start + d), k1 = __ldg(p.k_start + d + 1);
-        const uint32_t yes = __ballot_sync(0xffffffffu, in && min(max(q0, 0), p.q_rows) / run + d <= slot);
+        uint32_t yes;
+        int tile;
+        if (p.docs <= 32) {
+            // longest first: a document's slots follow those of all with more keys (of as many: with lower numbers)
+            const bool rows = in && q0 >= 0 && q1 > q0 && q1 <= p.q_rows;
+            const int runs = rows ? (q1 - q0 - 1) / run + 1 : 0, keys = max(k1, p.prefix) - max(k0, p.prefix);
+            int before = 0;
+            for (int o = 0; o < p.docs; ++o) {
+                const int other = __shfl_sync(0xffffffffu, keys, o), more = __shfl_sync(0xffffffffu, runs, o);
+                if (other > keys || (other == keys && o < lane))
+                    before += more;
+            }
+            tile = slot - before;
+            yes = __ballot_sync(0xffffffffu, tile >= 0 && tile < runs);
+        } else {
+            tile = slot - (q0 / run + d);
+            yes = __ballot_sync(0xffffffffu, in && min(max(q0, 0), p.q_rows) / run + d <= slot);
+        }
         const int k = yes ? 31 - __clz(yes) : 0;
         if (!yes || step == 1) {
             Document r;
-            r.index = yes ? lo + k : -1; // -1: rows before the first document
+            r.index = yes ? lo + k : -1;
+            r.tile = __shfl_sync(0xffffffffu, tile, k);
             r.q0 = __shfl_sync(0xffffffffu, q0, k), r.q1 = __shfl_sync(0xffffffffu, q1, k);
             r.k0 = __shfl_sync(0xffffffffu, k0, k), r.k1 = __shfl_sync(0xffffffffu, k1, k);
             return r;
@@ -155,8 +176,8 @@ __device__ __forceinline__ Run run_of(const PkArgs& p, int slot, int run_rows)
 {
     const Document doc = find_document(p, slot, run_rows);
     Run r;
-    r.row0 = doc.q0 + (slot - (doc.q0 / run_rows + doc.index)) * run_rows, r.q1 = doc.q1;
-    r.any = !(doc.index < 0 || doc.q0 < 0 || r.row0 < doc.q0 || r.row0 >= r.q1 || r.q1 > p.q_rows || doc.k0 < 0 || doc.k1 < doc.k0 ||
+    r.row0 = doc.q0 + doc.tile * run_rows, r.q1 = doc.q1;
+    r.any = !(doc.index < 0 || doc.q0 < 0 || doc.tile < 0 || r.row0 >= r.q1 || r.q1 > p.q_rows || doc.k0 < 0 || doc.k1 < doc.k0 ||
               doc.k1 > p.k_rows);
     r.a_end = p.prefix;
     r.b0 = max(doc.k0, p.prefix);
@@ -256,10 +277,10 @@ __global__ void __launch_bounds__(FEW_NT, 2) small_runs_kernel(const __grid_cons
     cluster_place(split, part);
     constexpr int STACK = BY_KEYS ? FEW_ROWS : FEW_ROWS * FEW_WARPS; // stacked rows of a run
     constexpr int SLICES = BY_KEYS ? 1 : FEW_KEYS / 16;              // 16-key slices of a block that a warp takes
-    const int kv_head = blockIdx.y, run_rows = STACK / p.group;
-    if (blockIdx.x == 0 && blockIdx.y == 0)
+    const int item = blockIdx.x / split, kv_head = item % p.kv_heads, run_rows = STACK / p.group;
+    if (blockIdx.x == 0)
         check_starts(p, FEW_NT);
-    const Run run = run_of(p, blockIdx.x / split, run_rows);
+    const Run run = run_of(p, item / p.kv_heads, run_rows);
     if (!run.any)
         return;
     const int a_blocks = (run.a_end + FEW_KEYS - 1) / FEW_KEYS;
@@ -904,9 +925,10 @@ __global__ void __launch_bounds__(NT, 1) packed_attention_kernel(const __grid_co
 {
     uint32_t split, part; // CTAs of this run's cluster, this one's number
     cluster_place(split, part);
-    if (blockIdx.x == 0 && blockIdx.y == 0)
+    if (blockIdx.x == 0)
         check_starts(p, NT);
-    const Run run = run_of(p, blockIdx.x / split, 4 * p.unit_rows);
+    const int item = blockIdx.x / split, kv_head = item % p.kv_heads;
+    const Run run = run_of(p, item / p.kv_heads, 4 * p.unit_rows);
     if (!run.any)
         return;
     const int a_blocks = (run.a_end + 127) / 128;
@@ -915,9 +937,9 @@ __global__ void __launch_bounds__(NT, 1) packed_attention_kernel(const __grid_co
     if (part >= split)
         return; // (a cluster barrier waits for the threads that are left)
     if (run.row0 + 2 * p.unit_rows < run.q1)
-        attend<HD, F16, true>(maps, p, run, blockIdx.y, split, part, a_blocks, blocks);
+        attend<HD, F16, true>(maps, p, run, kv_head, split, part, a_blocks, blocks);
     else
-        attend<HD, F16, false>(maps, p, run, blockIdx.y, split, part, a_blocks, blocks);
+        attend<HD, F16, false>(maps, p, run, kv_head, split, part, a_blocks, blocks);
 }
 
 CUtensorMap rows_map(const void* base, bool f16, int heads, int rows, int64_t stride, int head_dim, int box_heads, int box_rows)
@@ -938,10 +960,13 @@ void launch(const PackedAttnParams& p, const PkMaps& maps, const PkArgs& a, cuda
     c.attrs = at;
     c.numAttrs = 1;
     c.stream = s;
-    // Every run of every document has a slot: q_start[d] / rows + d is a document's first, and the last is under this.
+    // Every run of every document has a slot (a document of n rows has at most n / rows + 1 runs).
     auto grid = [&](int rows, int split) {
+        const long long ctas = ((long long)p.q_rows / rows + p.docs) * p.kv_heads * split;
+        if (ctas > 0x7fffffff)
+            throw std::invalid_argument("h3k_attention_packed: more runs of rows than a launch holds");
         at[0].val.clusterDim.x = unsigned(split);
-        c.gridDim = dim3(unsigned((long long)(p.q_rows / rows + p.docs) * split), p.kv_heads);
+        c.gridDim = dim3(unsigned(ctas));
     };
     const long long keys = p.prefix + (p.k_rows - p.prefix) / p.docs; // an average document's
     // The CTAs of a run's cluster: doubled while there are at most `room` in all and an average document would use half of
@@ -1000,7 +1025,7 @@ void attention_packed(const PackedAttnParams& p, cudaStream_t s)
     maps.v = p.k_rows > 0 ? rows_map(p.v, p.f16, p.kv_heads, p.k_rows, p.v_stride, p.head_dim, 1, 64) : maps.q;
     PkArgs a{};
     a.out = p.out, a.out_stride = p.out_stride, a.q_start = p.q_start, a.k_start = p.k_start, a.q_rows = p.q_rows, a.k_rows = p.k_rows;
-    a.docs = p.docs, a.prefix = p.prefix, a.group = group, a.unit_rows = unit_rows;
+    a.kv_heads = p.kv_heads, a.docs = p.docs, a.prefix = p.prefix, a.group = group, a.unit_rows = unit_rows;
     a.sl2 = float(double(p.scale) * 1.4426950408889634);
     if (p.head_dim == 128)
         (p.f16 ? launch<128, true> : launch<128, false>)(p, maps, a, s);
