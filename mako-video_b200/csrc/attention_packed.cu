@@ -972,7 +972,7 @@ void launch(const PackedAttnParams& p, const PkMaps& maps, const PkArgs& a, cuda
     // The CTAs of a run's cluster: doubled while there are at most `room` in all and an average document would use half of
     // them (`least` keys each); a run without the keys for all of them leaves some out.
     auto split_of = [&](int rows, int room, int least, int most) {
-        const long long runs = std::max<long long>(p.docs, (p.q_rows + rows - 1) / rows) * p.kv_heads;
+        const long long runs = std::max<long long>(p.docs, ((long long)p.q_rows + rows - 1) / rows) * p.kv_heads;
         int split = 1;
         while (split < most && runs * split * 2 <= room && keys >= (long long)split * least)
             split *= 2;
@@ -988,9 +988,13 @@ void launch(const PackedAttnParams& p, const PkMaps& maps, const PkArgs& a, cuda
             wide.fetch_or(device_bit());
         }
         const int rows = FEW_ROWS / a.group;
-        grid(rows, split_of(rows, 4 * num_sms(), FEW_LEAST * FEW_KEYS, FEW_SPLIT));
         c.blockDim = dim3(FEW_NT);
         c.dynamicSmemBytes = FewSmem<HD>::TOTAL;
+        int split = split_of(rows, 4 * num_sms(), FEW_LEAST * FEW_KEYS, FEW_SPLIT);
+        static ClusterLimits limits; // a cluster of more than eight is the device's to grant
+        if (split > 8 && limits.at_once(small_runs_kernel<HD, F16, true>, c, split) < 1)
+            split = 8;
+        grid(rows, split);
         H3_CUDA(cudaLaunchKernelEx(&c, small_runs_kernel<HD, F16, true>, maps, a, p.q, p.q_stride));
         return;
     }

@@ -50,13 +50,14 @@ void smem_opt_in(Kernel* kernel, int bytes, std::atomic<uint64_t>& done)
 // How many clusters of `size` CTAs of a kernel the current device holds at once (one object per kernel; asked once per
 // device and size). `c` describes the launch: block and shared memory, with the cluster dimension as its first attribute.
 struct ClusterLimits {
-    std::atomic<int> found[64][9] = {}; // + 1
+    static constexpr int kLargest = 16;
+    std::atomic<int> found[64][kLargest + 1] = {}; // + 1
     template <class Kernel>
     int at_once(Kernel* kernel, cudaLaunchConfig_t c, int size)
     {
         int dev = 0;
         cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
-        if (dev < 0 || dev > 63 || size < 1 || size > 8)
+        if (dev < 0 || dev > 63 || size < 1 || size > kLargest)
             return 0;
         int n = found[dev][size].load(std::memory_order_relaxed) - 1;
         if (n < 0) {
