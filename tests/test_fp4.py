@@ -409,3 +409,56 @@ def test_calls_in_a_graph_and_on_another_stream_repeat_bit_for_bit(cuda):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, -2 * first)
+
+
+# shapes by the form that the launch takes: K split over a cluster, CTAs that walk tiles of 128 rows, pairs of CTAs
+FORMS = {"split": (77, 1288, 1056), "split rows": (257, 512, 800), "tiles": (100, 38408, 96), "one tile": (128, 256, 256), "pairs": (300, 7176, 352), "pair edge": (513, 6416, 544)}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f", FORMATS)
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("epilogue", ["bf16", "f32", "gate", "swiglu"])
+def test_every_epilogue_in_every_form(cuda, f, form, epilogue):
+    M, N, K = FORMS[form]
+    if epilogue == "swiglu":
+        N = (N + 255) // 256 * 256
+    g = torch.Generator(device=cuda).manual_seed(M)
+    A, B = (gpu_quantise((torch.randn(n, K, generator=g, device=cuda) * s).bfloat16(), f) for n, s in ((M, 1.0), (N, 0.1)))
+    va, vb = (torch.from_numpy(F4.values(*F4.unpack(t[0].view(n, -1).cpu().numpy(), t[1].cpu().numpy(), f), None if t[2] is None else t[2].cpu().numpy(), f)).to(cuda)
+              for t, n in ((A, M), (B, N)))
+    bias = torch.randn(N, generator=g, device=cuda) * 0.1
+    y = va @ vb.T + bias.double()
+    t = K * 2.0 ** -23 * (va.abs() @ vb.abs().T) + 2.0 ** -22 * y.abs()
+    A, B = ((x[0].view(n, -1), x[1], x[2]) for x, n in ((A, M), (B, N)))
+    if epilogue == "gate":
+        mod, idx = torch.randn(2, 6, N, generator=g, device=cuda), (torch.arange(M, device=cuda) % 2).to(torch.uint8)
+        x = torch.randn(M + 1, N + 8, generator=g, device=cuda)
+        before, gate = x.clone(), mod[idx.long(), 2].double()
+        product(A, B, f, H.EPI_GATE_RESID, x=x, ldx=N + 8, bias=bias, mod=mod, mod_idx=idx, gate_slot=2, dim=N)
+        want = before[:M, :N].double() + gate * y
+        assert ((x[:M, :N] - want).abs() <= gate.abs() * t + 2.0 ** -23 * (want.abs() + (gate * y).abs())).all()
+        assert torch.equal(x[M], before[M]) and torch.equal(x[:, N:], before[:, N:])
+        return
+    low = epilogue != "f32"
+    if epilogue == "swiglu":
+        y, t = y.view(M, -1, 2, 128), t.view(M, -1, 2, 128)
+        gt, u, tg, tu = y[:, :, 0], y[:, :, 1], t[:, :, 0], t[:, :, 1]
+        y = (gt * sigmoid(gt) * u).reshape(M, -1)
+        t = (1.1 * tg * u.abs() + (gt * sigmoid(gt)).abs() * tu + tg * tu).reshape(M, -1) + 2.0 ** -20 * y.abs()
+    n = y.shape[1]
+    out = torch.full((M + 1, n + 8), 7.0, device=cuda, dtype=torch.bfloat16 if low else torch.float32)
+    product(A, B, f, {"bf16": H.EPI_BF16, "f32": H.EPI_F32, "swiglu": H.EPI_SWIGLU}[epilogue], out=out, ldo=n + 8, bias=bias)
+    assert ((out[:M, :n] - y).abs() <= t + (2.0 ** -8 * y.abs() if low else 0)).all()
+    assert (out[M] == 7).all() and (out[:, n:] == 7).all()
+
+
+@pytest.mark.gpu
+def test_product_without_bias_or_row_scales_and_one_row_of_any_pitch(cuda):
+    M, N, K, f = 1, 264, 544, F4.NV
+    A, B = operand(M, K, f, 1, cuda), operand(N, K, f, 2, cuda)
+    out = torch.full((N + 8,), 7.0, device=cuda)
+    product((A[0], A[1], None), (B[0], B[1], None), f, H.EPI_F32, out=out, ldo=3)  # one row: no pitch
+    want = (A[3] / A[2].double()[:, None]) @ (B[3] / B[2].double()[:, None]).T
+    tol = K * 2.0 ** -23 * ((A[3] / A[2].double()[:, None]).abs() @ (B[3] / B[2].double()[:, None]).abs().T)
+    assert ((out[:N] - want[0]).abs() <= tol[0]).all() and (out[N:] == 7).all()

@@ -116,7 +116,8 @@ def compare(out, want, tol):
 
 
 SELF = [([1], 0), ([1, 1, 1], 0), ([1, 1, 1], 1), ([5, 0, 130, 0], 5), ([256, 257, 3], 0), ([77, 300, 128, 64, 1000], 77), ([200, 1, 55, 129, 127], 200), ([0, 0, 7], 0),
-        ([128, 128, 384], 128), ([3] * 70, 3), ([1] * 1100, 0)]
+        ([128, 128, 384], 128), ([3] * 70, 3), ([1] * 1100, 0),
+        ([40] + [200] * 33 + [700, 0, 1], 40), ([5, 3000, 17, 1111, 640], 0)]
 
 
 @pytest.mark.gpu
