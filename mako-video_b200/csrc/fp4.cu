@@ -60,8 +60,8 @@ struct Run {
             }
         }
     }
-    // The bits of the largest magnitude as fp32 (an infinity or a NaN is larger than every number, a NaN than an
-    // infinity: magnitudes are compared as integers, which keeps both).
+    // The bits of the largest magnitude as fp32, a NaN if there is one (compared as integers, an infinity is larger than every
+    // number and a NaN than an infinity).
     __device__ __forceinline__ uint32_t largest() const
     {
         uint32_t m = 0;
@@ -71,11 +71,21 @@ struct Run {
                 m = max(m, w[i] & 0x7fffffffu);
             return m;
         } else {
+            if constexpr (T == Elem::bf16) {
+                __nv_bfloat162 b = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[0]));
 #pragma unroll
-            for (int i = 0; i < WORDS; ++i)
-                m = __vmaxu2(m, w[i] & 0x7fff7fffu);
-            m = max(m & 0xffffu, m >> 16);
-            return T == Elem::bf16 ? m << 16 : __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
+                for (int i = 1; i < WORDS; ++i)
+                    b = __hmax2_nan(b, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[i])));
+                m = *reinterpret_cast<uint32_t*>(&b);
+                return max(m & 0xffffu, m >> 16) << 16;
+            } else {
+                __half2 b = __habs2(*reinterpret_cast<const __half2*>(&w[0]));
+#pragma unroll
+                for (int i = 1; i < WORDS; ++i)
+                    b = __hmax2_nan(b, __habs2(*reinterpret_cast<const __half2*>(&w[i])));
+                m = *reinterpret_cast<uint32_t*>(&b);
+                return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(max(m & 0xffffu, m >> 16)))));
+            }
         }
     }
     __device__ __forceinline__ float2 pair(int i) const
@@ -292,7 +302,8 @@ __global__ void __launch_bounds__(256) dequant_fp4_kernel(const uint8_t* codes, 
         asm("{\n\t.reg .b8 lo, hi;\n\tmov.b16 {lo, hi}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, lo;\n\t}" : "=r"(h) : "h"(b));
         const float2 f = __half22float2(*reinterpret_cast<__half2*>(&h));
         // code x block scale is exact (2 and 4 bits), so the product with the row's scale is the one rounding in fp32
-        v[2 * i] = f.x * scale * g, v[2 * i + 1] = f.y * scale * g;
+        const float2 y = mul2(mul2(f, make_float2(scale, scale)), make_float2(g, g));
+        v[2 * i] = y.x, v[2 * i + 1] = y.y;
     }
     constexpr int WORDS = Run<T>::WORDS;
     uint32_t w[WORDS];

@@ -175,8 +175,9 @@ def test_quantise_bit_exact(cuda, f, kind, type, rows, K, ld):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("f", FORMATS)
-def test_quantise_says_nan_where_the_input_is_not_finite(cuda, f):
-    x = torch.ones(4, 128, dtype=torch.bfloat16, device=cuda)
+@pytest.mark.parametrize("type", list(TYPES))
+def test_quantise_says_nan_where_the_input_is_not_finite(cuda, f, type):
+    x = torch.ones(4, 128, dtype=TYPES[type][0], device=cuda)
     x[1, 40], x[2, 127], x[3, 0] = float("nan"), float("inf"), float("-inf")
     codes, tiles, row = gpu_quantise(x, f)
     want_codes, want_bytes, want_row, _ = F4.quantise(x.double().cpu().numpy(), f)
