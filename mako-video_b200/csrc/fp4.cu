@@ -182,12 +182,51 @@ __device__ __forceinline__ size_t scale_at(int row, int block, int tiles)
     return (size_t(row >> 7) * tiles + (block >> 2)) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
 }
 
+struct Packed {
+    uint8_t *codes, *scales;
+    int K, tiles;
+};
+
+// Run c of row r: its codes, and with its neighbours the word of their scales. All lanes of a warp, consecutive runs, a row of
+// the tensor's or, with scales of 0, one behind them that fills a scale tile; `in`: the row is the tensor's, `number`: it is finite (nv).
+template <Elem T, Fp4 F>
+__device__ __forceinline__ void store_run(const Packed& out, int r, int c, bool in, bool number, const Run<T>& a, uint32_t most, float rg)
+{
+    constexpr int PER = fp4_block(F) / 16; // runs of a block
+    if constexpr (F == Fp4::mx)
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1)); // the block's other half (both in the row: K is a multiple of 32)
+    uint32_t byte = 0;
+    uint2 code = make_uint2(0, 0);
+    const bool have = in && c < out.K / 16;
+    if (have && number)
+        code = encode<T, F>(a, most, rg, byte);
+    if (have)
+        *reinterpret_cast<uint2*>(out.codes + size_t(r) * (out.K / 2) + size_t(c) * 8) = code;
+    // four lanes' (eight for mx) bytes into one word
+    uint32_t word = byte << (8 * ((c / PER) & 3));
+#pragma unroll
+    for (int o = PER; o < 4 * PER; o <<= 1)
+        word |= __shfl_xor_sync(0xffffffffu, word, o);
+    if (c < out.tiles * 4 * PER && (c & (4 * PER - 1)) == 0)
+        *reinterpret_cast<uint32_t*>(out.scales + scale_at(r, c / PER, out.tiles)) = word;
+}
+
+// The scale of an nv row whose largest magnitude has the bits `most`: 2^(floor(log2 max) - 10), which makes block scales up to
+// 2^11 / 6 = 341.3, under e4m3's 448. Returns its reciprocal; not a number: 0, and a NaN for the scale.
+__device__ __forceinline__ float row_scale_of(uint32_t most, float& scale)
+{
+    const int e = max(int(most >> 23) - 127 - 10, -126);
+    const bool number = most < 0x7f800000u;
+    scale = number ? power_of_two(e) : __uint_as_float(0x7fffffffu);
+    return number ? power_of_two(-e) : 0.f;
+}
+
 constexpr int QUANT_RUNS = 2;    // runs of 16 values that a thread keeps: few, so that many threads have loads under way
 constexpr int QUANT_THREADS = 512; // of a CTA at most
 
 // blockDim.x = 32 x the warps of a row (RUNS runs a thread; a row of more runs than that is read twice instead of kept), or,
 // for SHORT rows of one warp, of as many rows.
-// (64 registers a thread: 33024 x 5120 in 86 us for nv and 68 for mx; unbounded, with 72, 98 and 70.)
+// (64 registers a thread: 33024 x 5120 in 88 us for nv and 67 for mx; unbounded, with 72, 98 and 70.)
 template <Elem T, Fp4 F, bool SHORT>
 __global__ void __launch_bounds__(QUANT_THREADS, 2) quant_fp4_kernel(const void* x, int64_t ldx, int rows, int K, bool wide, uint8_t* codes,
                                                                   uint8_t* scales, float* row_scale)
@@ -230,40 +269,20 @@ __global__ void __launch_bounds__(QUANT_THREADS, 2) quant_fp4_kernel(const void*
             __syncthreads();
             all = __reduce_max_sync(0xffffffffu, lane_id() < int(blockDim.x) / 32 ? red[lane_id()] : 0);
         }
-        // 2^(floor(log2 max) - 10): block scales up to 2^11 / 6 = 341.3, under e4m3's 448
-        const int e = max(int(all >> 23) - 127 - 10, -126);
-        const bool number = all < 0x7f800000u;
-        rg = number ? power_of_two(-e) : 0.f;
+        float scale;
+        rg = row_scale_of(all, scale);
         if (in && t == 0)
-            row_scale[r] = number ? power_of_two(e) : __uint_as_float(0x7fffffffu);
+            row_scale[r] = scale;
     }
     const bool number = F == Fp4::mx || all < 0x7f800000u;
     // The runs come in whole tiles of four scale bytes (2 runs a byte for mx); the tail's bytes and the rows past the
     // tensor's are 0.
     const int padded = tiles * 4 * fp4_block(F) / 16;
-    auto finish = [&](int c, const Run<T>& a, uint32_t m) {
-        uint32_t byte = 0;
-        uint2 code = make_uint2(0, 0);
-        const bool have = in && c < runs;
-        if constexpr (F == Fp4::mx)
-            m = max(m, __shfl_xor_sync(0xffffffffu, m, 1)); // the block's other half (both in the row: K is a multiple of 32)
-        if (have && number)
-            code = encode<T, F>(a, m, rg, byte);
-        if (have)
-            *reinterpret_cast<uint2*>(codes + size_t(r) * (K / 2) + size_t(c) * 8) = code;
-        // four lanes' (eight for mx) bytes into one word
-        constexpr int PER = fp4_block(F) / 16;
-        uint32_t word = byte << (8 * ((c / PER) & 3));
-#pragma unroll
-        for (int o = PER; o < 4 * PER; o <<= 1)
-            word |= __shfl_xor_sync(0xffffffffu, word, o);
-        if (c < padded && (c & (4 * PER - 1)) == 0 && (r >> 7) < (rows + 127) >> 7)
-            *reinterpret_cast<uint32_t*>(scales + scale_at(r, c / PER, tiles)) = word;
-    };
+    const Packed out{codes, scales, K, tiles};
 #pragma unroll
     for (int i = 0; i < RUNS; ++i)
         if (i * step < padded) // the same for the whole CTA: the shuffles see full warps
-            finish(t + i * step, keep[i], most[i]);
+            store_run<T, F>(out, r, t + i * step, in, number, keep[i], most[i], rg);
     for (int c0 = RUNS * step; c0 < padded; c0 += step) {
         const int c = c0 + t;
         Run<T> a;
@@ -272,7 +291,78 @@ __global__ void __launch_bounds__(QUANT_THREADS, 2) quant_fp4_kernel(const void*
             a.load(row, c * 16, wide);
             m = a.largest();
         }
-        finish(c, a, m);
+        store_run<T, F>(out, r, c, in, number, a, m, rg);
+    }
+}
+
+// Long nv rows of 16-bit values: few CTAs of that many threads fit an SM, and all of them wait for a row's last value before
+// they go on. So CTAs stay and walk rows, which bulk copies bring into shared memory ahead of them: 33024 x 13824 in 230 us
+// against 270, x 8224 in 146 against 166; at 5120 the two take the same, below it this one loses.
+constexpr int RING = 3; // rows
+template <Elem T>
+__global__ void __launch_bounds__(QUANT_THREADS, 2) quant_long_rows_kernel(const void* x, int64_t ldx, int rows, int K, uint8_t* codes, uint8_t* scales,
+                                                                        float* row_scale)
+{
+    static_assert(T != Elem::f32);
+    constexpr int RUNS = QUANT_RUNS;
+    extern __shared__ __align__(128) uint8_t ring[]; // [RING][K] values
+    __shared__ uint32_t red[2][QUANT_THREADS / 32];
+    __shared__ uint64_t full[RING];
+    const int step = blockDim.x, t = threadIdx.x;
+    const int runs = K / 16;
+    const Packed out{codes, scales, K, fp4_scale_tiles(K, Fp4::nv)};
+    const int all_rows = (rows + 127) / 128 * 128; // the rows behind the tensor's have scales of 0
+    const uint32_t bytes = uint32_t(K) * 2;
+    auto fetch = [&](int64_t r, int turn) {
+        if (r < rows) {
+            mbar_arrive_expect_tx(&full[turn % RING], bytes);
+            bulk_load(ring + (turn % RING) * bytes, static_cast<const uint8_t*>(x) + size_t(r) * ldx * 2, bytes, &full[turn % RING]);
+        }
+    };
+    if (t == 0) {
+        for (int i = 0; i < RING; ++i)
+            mbar_init(&full[i], 1);
+        fence_barrier_init();
+        for (int i = 0; i < RING; ++i)
+            fetch(int64_t(blockIdx.x) + int64_t(i) * gridDim.x, i);
+    }
+    __syncthreads();
+    int turn = 0;
+    for (int64_t r = blockIdx.x; r < all_rows; r += gridDim.x, ++turn) {
+        const bool in = r < rows;
+        if (in && !mbar_wait(&full[turn % RING], (turn / RING) & 1))
+            return; // (the device error is set; this CTA's copies have had seconds to land)
+        const uint4* row = reinterpret_cast<const uint4*>(ring + (turn % RING) * bytes);
+        Run<T> keep[RUNS];
+        uint32_t most[RUNS], all = 0;
+#pragma unroll
+        for (int i = 0; i < RUNS; ++i) {
+            most[i] = 0;
+            if (in && t + i * step < runs) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const uint4 v = row[(t + i * step) * 2 + j];
+                    keep[i].w[4 * j] = v.x, keep[i].w[4 * j + 1] = v.y, keep[i].w[4 * j + 2] = v.z, keep[i].w[4 * j + 3] = v.w;
+                }
+                most[i] = keep[i].largest();
+                all = max(all, most[i]);
+            }
+        }
+        all = __reduce_max_sync(0xffffffffu, all);
+        if (lane_id() == 0)
+            red[turn & 1][warp_id()] = all;
+        __syncthreads(); // the row is in registers, and the warps' maxima are there
+        if (t == 0)
+            fetch(r + int64_t(RING) * gridDim.x, turn);
+        all = __reduce_max_sync(0xffffffffu, lane_id() < int(blockDim.x) / 32 ? red[turn & 1][lane_id()] : 0);
+        float scale;
+        const float rg = row_scale_of(all, scale);
+        if (in && t == 0)
+            row_scale[r] = scale;
+#pragma unroll
+        for (int i = 0; i < RUNS; ++i)
+            if (i * step < out.tiles * 4)
+                store_run<T, Fp4::nv>(out, int(r), t + i * step, in, all < 0x7f800000u, keep[i], most[i], rg);
     }
 }
 
@@ -344,6 +434,16 @@ void quant(const void* x, int64_t ldx, int rows, int K, void* codes, void* scale
     auto* c = static_cast<uint8_t*>(codes);
     auto* sc = static_cast<uint8_t*>(scales);
     const int warps = (runs + 32 * QUANT_RUNS - 1) / (32 * QUANT_RUNS);
+    if constexpr (F == Fp4::nv && T != Elem::f32) {
+        const int threads = 32 * warps, ctas = num_sms() * std::max(1, 1024 / threads); // with 64 registers a thread
+        if (warps > 8 && threads <= QUANT_THREADS && all_rows >= 2 * ctas) {
+            static std::atomic<uint64_t> opt_in;
+            smem_opt_in(quant_long_rows_kernel<T>, RING * 32 * QUANT_RUNS * QUANT_THREADS, opt_in);
+            quant_long_rows_kernel<T><<<ctas, threads, RING * K * 2, s>>>(x, ldx, rows, K, c, sc, row_scale);
+            H3_CUDA(cudaGetLastError());
+            return;
+        }
+    }
     if (warps == 1) // eight rows a CTA
         quant_fp4_kernel<T, F, true><<<all_rows / 8, 256, 0, s>>>(x, ldx, rows, K, wide, c, sc, row_scale);
     else
