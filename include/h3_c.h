@@ -405,8 +405,8 @@ int h3k_fp4_sizes(int32_t rows, int32_t K, int32_t format, uint64_t* code_bytes,
  * scale (MX) or its row's (NV) a NaN, with codes of 0. row_scale: NULL for MX. */
 int h3k_quant_rows_fp4(const void* x, int32_t type, int64_t ldx, int32_t rows, int32_t K, int32_t format, void* codes, void* scales,
                        float* row_scale, void* stream);
-/* The values that the codes stand for, code x block scale x row scale, rounded once to `type`; out's rows ldo apart.
- * row_scale NULL: 1. */
+/* The values that the codes stand for, code x block scale x row scale (in fp32: exact with a power of two for a row scale,
+ * as the quantiser's are), rounded to `type`; out's rows ldo apart. row_scale NULL: 1. */
 int h3k_dequant_rows_fp4(const void* codes, const void* scales, const float* row_scale, int32_t rows, int32_t K, int32_t format, int32_t type,
                          void* out, int64_t ldo, void* stream);
 /* D[M][N] = A[M][K] B[N][K]^T of two such matrices of one format, fp32 accumulation, with h3k_gemm's epilogues (0 to 4) and

@@ -36,7 +36,10 @@ constexpr float kRescaleThreshold = 8.0f;  // log2 units
 // one is a third V slot.
 constexpr int KST = 3, VST = 2;
 constexpr int NT = 64 + 256;
-constexpr int LEAST = 4; // 128-key blocks that a CTA takes before another one joins it
+// 128-key blocks of a CTA's before more of its cluster join in, and of theirs at least: a block takes 2.3 us, writing, joining and
+// storing the parts of 256 rows about 8 (600 rows and keys of 10 heads in 16.3 us by one CTA, 19.3 by two; 3000 keys in 24.5 by
+// six, 30.2 by three).
+constexpr int LEAST = 4;
 
 template <int HD>
 struct PkSmem {
@@ -876,43 +879,72 @@ __device__ __forceinline__ void attend(const PkMaps& maps, const PkArgs& p, cons
         tmem_dealloc(tmem, 512);
     }
     if (join) {
-        // A warp a row, the rows dealt out over the cluster's CTAs; parts weighted by 2^(m_part - max), in their order.
+        // A warp four rows at a time, whose loads are under way together, the rows dealt out over the cluster's CTAs; parts
+        // weighted by 2^(m_part - max), in their order.
         if (split > 1)
             cluster_sync();
-        const int rows = TWO ? 256 : 128, tiles = TWO ? 1 : 2; // tiles: parts of a row in a CTA
-        for (int r = int(part) + warp * int(split); r < rows; r += int(split) * (NT / 32)) {
-            const int in_unit = r & 63;
-            const int out_row = row0 + (r >> 6) * p.unit_rows + in_unit / p.group;
-            if (in_unit >= p.unit_rows * p.group || out_row >= q1)
-                continue;
-            const int parts = int(split) * tiles;
-            // lane z holds part z's (max, sum): CTA z / tiles, tile z % tiles
-            float2 a = make_float2(-INFINITY, 0.f);
-            if (lane_id() < parts)
-                a = ld_cluster2(smem_u32(smem) + (lane_id() % tiles * 128 + r) * 8, lane_id() / tiles);
-            float mx = a.x;
+        constexpr int AT_ONCE = 4;
+        constexpr int tiles = TWO ? 1 : 2, all_rows = TWO ? 256 : 128; // tiles: parts of a row in a CTA
+        const int parts = int(split) * tiles, lane = lane_id();
+        const int piece = lane < HD / 4 ? lane : 0;
+        const int step = int(split) * (NT / 32);
+        for (int r0 = int(part) + warp * int(split); r0 < all_rows; r0 += step * AT_ONCE) {
+            auto place = [&](int u, int& out_row, int& in_unit) {
+                const int r = r0 + u * step;
+                in_unit = r & 63;
+                out_row = row0 + (r >> 6) * p.unit_rows + in_unit / p.group;
+                return r < all_rows && in_unit < p.unit_rows * p.group && out_row < q1;
+            };
+            float2 a[AT_ONCE]; // lane z: part z's (max, sum), of CTA z / tiles and tile z % tiles
+            bool any = false;
 #pragma unroll
-            for (int o = 8; o > 0; o >>= 1)
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o, 16));
-            mx = __shfl_sync(0xffffffffu, mx, 0);
-            const float w_part = a.y == 0.f ? 0.f : ex2_approx(a.x - (mx == -INFINITY ? 0.f : mx));
-            float sum = 0.f;
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            const int piece = lane_id() < HD / 4 ? lane_id() : 0;
-#pragma unroll 4
-            for (int z = 0; z < parts; ++z) {
-                const float w = __shfl_sync(0xffffffffu, w_part, z), l = __shfl_sync(0xffffffffu, a.y, z);
-                if (l == 0.f)
-                    continue; // a part without keys has written no row
-                const int at = z % tiles * 128 + r;
-                const float4 v = ld_cluster4(smem_u32(smem + OFF_K) + at * HD * 4 + ((piece ^ (at & 7)) << 4), z / tiles);
-                sum += w * l;
-                acc.x += w * v.x, acc.y += w * v.y, acc.z += w * v.z, acc.w += w * v.w;
+            for (int u = 0; u < AT_ONCE; ++u) {
+                int out_row, in_unit;
+                a[u] = make_float2(-INFINITY, 0.f);
+                if (place(u, out_row, in_unit)) {
+                    any = true;
+                    if (lane < parts)
+                        a[u] = ld_cluster2(smem_u32(smem) + (lane % tiles * 128 + r0 + u * step) * 8, lane / tiles);
+                }
             }
-            const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-            if (lane_id() < HD / 4) {
+            if (!any)
+                continue;
+            float w[AT_ONCE], sum[AT_ONCE];
+            float4 acc[AT_ONCE];
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+                float mx = a[u].x;
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1)
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                w[u] = a[u].y == 0.f ? 0.f : ex2_approx(a[u].x - (mx == -INFINITY ? 0.f : mx));
+                sum[u] = w[u] * a[u].y;
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1)
+                    sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], o);
+                sum[u] = __shfl_sync(0xffffffffu, sum[u], 0);
+                acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll 2
+            for (int z = 0; z < parts; ++z)
+#pragma unroll
+                for (int u = 0; u < AT_ONCE; ++u) {
+                    const float wz = __shfl_sync(0xffffffffu, w[u], z);
+                    if (wz == 0.f)
+                        continue; // a part without keys has written no row, and no row has no part
+                    const int at = z % tiles * 128 + r0 + u * step;
+                    const float4 v = ld_cluster4(smem_u32(smem + OFF_K) + at * HD * 4 + ((piece ^ (at & 7)) << 4), z / tiles);
+                    acc[u].x += wz * v.x, acc[u].y += wz * v.y, acc[u].z += wz * v.z, acc[u].w += wz * v.w;
+                }
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+                int out_row, in_unit;
+                if (!place(u, out_row, in_unit) || lane >= HD / 4)
+                    continue;
+                const float inv = sum[u] > 0.f ? 1.f / sum[u] : (sum[u] == 0.f ? 0.f : sum[u]);
                 uint16_t* dst = static_cast<uint16_t*>(p.out) + size_t(out_row) * p.out_stride + (kv_head * p.group + in_unit % p.group) * HD;
-                *reinterpret_cast<uint2*>(dst + piece * 4) = make_uint2(pack2<F16>(acc.x * inv, acc.y * inv), pack2<F16>(acc.z * inv, acc.w * inv));
+                *reinterpret_cast<uint2*>(dst + piece * 4) =
+                    make_uint2(pack2<F16>(acc[u].x * inv, acc[u].y * inv), pack2<F16>(acc[u].z * inv, acc[u].w * inv));
             }
         }
         if (split > 1)
@@ -933,7 +965,7 @@ __global__ void __launch_bounds__(NT, 1) packed_attention_kernel(const __grid_co
         return;
     const int a_blocks = (run.a_end + 127) / 128;
     const int blocks = a_blocks + (run.b_end - run.b0 + 127) / 128;
-    split = parts_of(blocks, LEAST, split);
+    split = blocks < 2 * LEAST ? 1 : parts_of(blocks, LEAST, split);
     if (part >= split)
         return; // (a cluster barrier waits for the threads that are left)
     if (run.row0 + 2 * p.unit_rows < run.q1)

@@ -36,7 +36,7 @@ inline size_t fp4_scale_bytes(int rows, int K, Fp4 f) { return size_t((rows + 12
 // scale bytes, padding included; row_scale [rows] for nv only.
 void quant_rows_fp4(const void* x, Elem type, int64_t ldx, int rows, int K, Fp4 f, void* codes, void* scales, float* row_scale,
                     cudaStream_t s);
-// The values that the codes stand for, rounded once to the output's type (rows ldo elements apart, 16-byte aligned).
+// The values that the codes stand for, in fp32 and rounded to the output's type (rows ldo elements apart, 16-byte aligned).
 // row_scale null: 1.
 void dequant_rows_fp4(const void* codes, const void* scales, const float* row_scale, int rows, int K, Fp4 f, Elem type, void* out,
                       int64_t ldo, cudaStream_t s);

@@ -1,17 +1,20 @@
 // The projection GEMM on microscaled 4-bit rows (layouts in fp4.cuh): tcgen05.mma kind::mxf4 / kind::mxf4nvf4 with the
 // block scales in TMEM, fp32 accumulation, the row scales and the step's epilogues on the way out.
 //
-// One CTA per SM: warp 0 loads (TMA tiles of 128 bytes = 256 values of K, 128-byte swizzled; the scale tiles by plain bulk
-// copies), warp 1 issues, warps 2..9 are the epilogue. Per stage the issuer copies the stage's scale tiles from shared
-// memory into TMEM (tcgen05.cp, in order before the MMAs that read them) and runs four MMAs of K = 64 and 128 rows x 256
-// columns per SM. The issue itself is what a stage's 12 copies and 4 MMAs in 512 clocks strain: descriptors are made once a
-// stage and the warp stays converged (one lane chosen by elect.sync), which took 33024 x 15360 x 5120 without an epilogue
-// from 1.68 ms to 0.93.
+// One CTA per SM: warp 0 loads (TMA tiles of 128 bytes = 256 values of K, 128-byte swizzled, and the scale tiles as they lie),
+// warp 1 issues, warps 2..9 are the epilogue. Per stage the issuer copies the stage's scale tiles from shared memory into
+// TMEM (tcgen05.cp, in order before the MMAs that read them) and runs four MMAs of K = 64 and 128 rows x 256 columns per SM.
+// The issue itself is what a stage's 12 copies and 4 MMAs in 512 clocks strain: descriptors are made once a stage and the
+// warp stays converged (one lane chosen by elect.sync), which took the main loop of 33024 x 15360 x 5120 from 1.68 ms to
+// 0.93 (before the pairs).
 //
 // Three forms:
 //   pair   (more than 128 rows) the two CTAs of a cluster share a tile of 256 x 256: each loads its 128 rows of A and half of
-//          B's, the first CTA issues for both (cta_group::2). A stage is 38 KB instead of 54 and five fit, which matters
-//          because at 54 KB in 512 clocks an SM's share of the L2 bandwidth, not the tensor core, sets the pace.
+//          B's, the first CTA issues for both (cta_group::2). A stage is 38 KB instead of 54 and five fit: at 54 KB in 512
+//          clocks an SM's share of the L2 bandwidth, not the tensor core, sets the pace. 33024 x 15360 x 5120 takes 0.97 ms
+//          (5.4 PFLOP/s; tensor pipe 77% at the 1.45 GHz that the power limit leaves) against 1.19 in single CTAs, about
+//          0.13 of it the output's stores. The second CTA's loads complete on the first one's barriers; its thread
+//          telling the first by a remote arrival a stage took 1.5 ms.
 //   tiles  (at most 128 rows) a CTA walks tiles of 128 x 256
 //   split  (fewer such tiles than half the SMs) the K of a tile is split over the CTAs of a cluster; they leave their sums in
 //          shared memory and each finishes a share of the tile from all of them, in their order
@@ -228,8 +231,8 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr, uint32_t rank)
 // g / (1 + e^-g); the quotient within 2 ulp (0 once e^-g is above 2^126, where it is below 2^-119)
 __device__ __forceinline__ float silu_approx(float g) { return __fdividef(g, 1.0f + __expf(-g)); }
 
-// First of the columns [half 0: 0, half 1: 64) ... that an epilogue thread's 32-column chunk c of 4 holds, within the tile. The
-// SwiGLU pairs gate column j with value column 128 + j, so a thread takes 64 of both; else 128 columns in a row.
+// First column, within the tile, of the chunk c (of four of 32 columns) that an epilogue thread of a half holds: the SwiGLU
+// pairs gate column j with value column 128 + j, so a thread takes 64 of both; else 128 columns in a row.
 template <Epi EPI>
 __device__ __forceinline__ int chunk_col(int half, int c)
 {

@@ -143,18 +143,25 @@ def rows_like(rows, K, seed, kind="normal"):
     return x
 
 
-# many long rows: 1201 are walked by CTAs that stay
-LONG = [(1201, 8224, 8232), (1201, 16384, 16384)]
-
-
 @pytest.mark.gpu
 @pytest.mark.parametrize("f", FORMATS)
 @pytest.mark.parametrize("kind", ["normal", "ties", "wide"])
 @pytest.mark.parametrize("type", list(TYPES))
-@pytest.mark.parametrize("rows,K,ld", [(1, 32, 32), (3, 96, 104), (130, 160, 160), (33, 2048, 2048), (5, 4160, 4224), (7, 8224, 8224), (2, 16416, 16416), (3, 40000, 40000)] + LONG)
+@pytest.mark.parametrize("rows,K,ld", [(1, 32, 32), (3, 96, 104), (130, 160, 160), (33, 2048, 2048), (5, 4160, 4224), (7, 8224, 8224), (2, 16416, 16416), (3, 40000, 40000)])
 def test_quantise_bit_exact(cuda, f, kind, type, rows, K, ld):
-    if (rows, K, ld) in LONG and (f == F4.MX or kind == "ties"):
-        pytest.skip("long rows of many are nv's")
+    check_quantise(cuda, f, kind, type, rows, K, ld)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["normal", "wide"])
+@pytest.mark.parametrize("type", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,K,ld", [(1201, 8224, 8232), (1201, 16384, 16384)])
+def test_quantise_many_long_rows_bit_exact(cuda, kind, type, rows, K, ld):
+    """Rows that CTAs walk instead of having one each."""
+    check_quantise(cuda, F4.NV, kind, type, rows, K, ld)
+
+
+def check_quantise(cuda, f, kind, type, rows, K, ld):
     dtype = TYPES[type][0]
     x = torch.from_numpy(rows_like(rows, ld, rows + K, kind)).clamp(-3e38, 3e38).to(dtype)
     x = x.clamp(-torch.finfo(dtype).max, torch.finfo(dtype).max).to(cuda)
