@@ -389,8 +389,8 @@ int h3k_layer_norm(const float* x, int32_t rows, int32_t d, const float* w, cons
  *              blocks past the matrix are part of the buffer and must be 0 (the quantiser writes them)
  *   row_scale  fp32 [rows], H3K_FP4_NV only
  * H3K_FP4_MX: blocks of 32, scale 2^e as byte e + 127 (255: NaN). H3K_FP4_NV: blocks of 16, e4m3 scales.
- * All pointers are device memory of the current device, 16-byte aligned (row_scale 4); work is queued on `stream`, and
- * the calls may be captured into a graph. 0 rows: nothing is done. */
+ * All pointers are device memory of the current device, 16-byte aligned (row_scale 4), an output's apart from the others';
+ * work is queued on `stream`, and the calls may be captured into a graph. At most 2^31 - 128 rows; 0: nothing is done. */
 #define H3K_FP4_MX 0
 #define H3K_FP4_NV 1
 #define H3K_BF16 0 /* element types */
@@ -440,7 +440,7 @@ typedef struct h3k_packed_args {
                             /* which what the call wrote is not to be used; nothing outside the rows is touched */
     float scale;            /* 0: 1 / sqrt(head_dim) */
 } h3k_packed_args;
-/* Queued on `stream`, no scratch and no synchronisation; may be captured into a graph. */
+/* out overlaps none of the others. Queued on `stream`, no scratch and no synchronisation; may be captured into a graph. */
 int h3k_attention_packed(const h3k_packed_args* args, void* stream);
 
 #ifdef __cplusplus

@@ -51,9 +51,12 @@ h3::Fp4 to_format(const char* call, int32_t format)
     return h3::Fp4(format);
 }
 
+constexpr int32_t kMostRows = 0x7fffff80; // in whole scale tiles of 128 rows, still an int
+
 void check_rows(const char* call, int32_t rows, int32_t K)
 {
     need(rows >= 0, call, "a negative number of rows");
+    need(rows <= kMostRows, call, "more than 2^31 - 128 rows");
     need(K > 0 && K % 32 == 0, call, "K must be a positive multiple of 32");
 }
 
@@ -121,6 +124,7 @@ int h3k_gemm_fp4(const void* A, const void* A_scales, const void* B, const void*
         need(a, call, "null argument");
         check_rows(call, a->M, a->K);
         need(a->N > 0 && a->N % 8 == 0, call, "N must be a positive multiple of 8");
+        need(a->N <= kMostRows, call, "more than 2^31 - 128 columns");
         need(epilogue >= H3K_EPI_BF16 && epilogue <= H3K_EPI_SWIGLU, call, "unknown epilogue");
         need(a->a_chunks <= 1 && a->a_rows_stride == 0 && (a->lda == 0 || a->lda == a->K) && (a->ldb == 0 || a->ldb == a->K), call,
              "packed rows are contiguous: no chunks or pitches");

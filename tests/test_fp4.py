@@ -107,6 +107,17 @@ def test_product_refuses_null_operands_and_a_wrong_format():
     refused(L.h3k_gemm_fp4(BASE, BASE, BASE, BASE, F4.MX, None, H.EPI_BF16, None), "null")
 
 
+def test_more_rows_than_whole_scale_tiles_can_number_are_refused():
+    L, most = H.lib(), 0x7fffff80
+    assert H.fp4_sizes(most, 32, F4.MX) == (most * 16, most // 128 * 512)
+    refused(L.h3k_fp4_sizes(most + 1, 32, F4.MX, None, None), "rows")
+    refused(L.h3k_quant_rows_fp4(BASE, H.BF16, 0, most + 1, 32, F4.MX, BASE, BASE, None, None), "rows")
+    refused(L.h3k_dequant_rows_fp4(BASE, BASE, None, most + 1, 32, F4.MX, H.BF16, BASE, 32, None), "rows")
+    for change, text in ((dict(M=most + 1), "rows"), (dict(N=most + 8), "columns")):
+        a = H.h3k_gemm_args(**(dict(M=3, N=256, K=64, out=BASE, ldo=256) | change))
+        refused(L.h3k_gemm_fp4(BASE, BASE, BASE, BASE, F4.MX, ctypes.byref(a), H.EPI_BF16, None), text)
+
+
 def test_no_rows_is_no_work():
     L = H.lib()
     assert L.h3k_quant_rows_fp4(None, H.BF16, 64, 0, 64, F4.MX, None, None, None, None) == H.H3_OK
