@@ -9,15 +9,16 @@
 // 0.93 (before the pairs).
 //
 // Three forms:
-//   pair   (more than 128 rows) the two CTAs of a cluster share a tile of 256 x 256: each loads its 128 rows of A and half of
+//   pair   (more than 128 rows, or few tiles) the two CTAs of a cluster share a tile of 256 x 256: each loads its 128 rows of A and half of
 //          B's, the first CTA issues for both (cta_group::2). A stage is 38 KB instead of 54 and five fit: at 54 KB in 512
 //          clocks an SM's share of the L2 bandwidth, not the tensor core, sets the pace. 33024 x 15360 x 5120 takes 0.97 ms
 //          (5.4 PFLOP/s; tensor pipe 77% at the 1.45 GHz that the power limit leaves) against 1.19 in single CTAs, about
 //          0.13 of it the output's stores. The second CTA's loads complete on the first one's barriers; its thread
 //          telling the first by a remote arrival a stage took 1.5 ms.
-//   tiles  (at most 128 rows) a CTA walks tiles of 128 x 256
-//   split  (fewer such tiles than half the SMs) the K of a tile is split over the CTAs of a cluster; they leave their sums in
-//          shared memory and each finishes a share of the tile from all of them, in their order
+//   tiles  (at most 128 rows, more tiles of 128 x 256 than half the SMs) a CTA walks such tiles: 1 row of 27648 columns and
+//          K = 5120 in 22.8 us against 28.8 by pairs, whose second CTA would have no rows
+//   split  (fewer such tiles, of few rows or long K: the rule is in launch()) the K of a tile is split over the CTAs of a
+//          cluster; they leave their sums in shared memory and each finishes a share of the tile from all of them, in order
 //
 // TMEM: the accumulator's 256 columns, then the scales of every stage of the ring (48 columns each for nv), so that a stage's
 // `empty` barrier covers its scales too; a second accumulator would leave none of the 512 for them. The epilogue's eight
@@ -631,12 +632,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 continue;
             auto sum = [&](int piece) {
                 const uint32_t at = smem_u32(smem) + (r * (BN / 4) + (piece ^ (r & 7))) * 16;
-                float4 s = ld_cluster4(at, 0);
-                for (uint32_t z = 1; z < split; ++z) {
-                    const float4 v = ld_cluster4(at, z);
-                    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
-                }
-                return s;
+                float4 v[MAX_SPLIT]; // loads under way together
+#pragma unroll
+                for (uint32_t z = 0; z < MAX_SPLIT; ++z)
+                    v[z] = z < split ? ld_cluster4(at, z) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (uint32_t z = 1; z < MAX_SPLIT; ++z)
+                    v[0].x += v[z].x, v[0].y += v[z].y, v[0].z += v[z].z, v[0].w += v[z].w;
+                return v[0];
             };
             const float4 s = sum(g);
             finish4<EPI>(p, s, EPI == Epi::swiglu ? sum(g + 32) : s, tm * BM + r, col);
@@ -709,7 +712,12 @@ bool launch(const void* A, const void* a_scales, const void* B, const void* b_sc
         for (split = std::min({ctas / tiles, MAX_SPLIT, (p.K + KSTAGE - 1) / KSTAGE}); split > 1; --split)
             if (limits.at_once(gemm_fp4_kernel<EPI, F, W>, c, split) >= tiles)
                 break;
-        if (split < 2)
+        // Against pairs of 128 columns a CTA, with which a stage takes 0.31 us instead of 0.6 (its share of B is half, the ring
+        // deeper): the parts' sums take 4 us through the cluster's shared memory for 128 rows and nearly none for one. K = 5120:
+        // 1 row of 5120 columns takes 9.1 us by seven parts and 12.5 by pairs, 64 rows 11.1 and 12.6, 128 rows 13.3 and 13.0;
+        // 128 rows of 15360 columns 18.4 by two parts and 14.9 by pairs.
+        const long long stages = (p.K + KSTAGE - 1) / KSTAGE;
+        if (split < 2 || stages * (split - 2) * 8 <= (long long)(std::min(p.M, BM) - 32) * split)
             return false;
         at[0].val.clusterDim.x = unsigned(split);
         ctas = tiles * split;
@@ -727,7 +735,7 @@ void run(const void* A, const void* a_scales, const void* B, const void* b_scale
     if constexpr (EPI != Epi::qkv) // its norm runs along whole rows of a tile
         if (tiles * 2 <= sms && p.K > KSTAGE && launch<EPI, F, Form::split>(A, a_scales, B, b_scales, p, int(tiles), sms, s))
             return;
-    if (p.M > BM) {
+    if (p.M > BM || tiles * 2 <= sms) {
         const long long pairs = (p.M + 2 * BM - 1) / (2 * BM) * tiles_n;
         launch<EPI, F, Form::pair>(A, a_scales, B, b_scales, p, int(pairs), int(std::min<long long>(pairs, sms / 2)) * 2, s);
     } else {

@@ -437,7 +437,9 @@ def test_calls_in_a_graph_and_on_another_stream_repeat_bit_for_bit(cuda):
 
 
 # shapes by the form that the launch takes: K split over a cluster, CTAs that walk tiles of 128 rows, pairs of CTAs
-FORMS = {"split": (77, 1288, 1056), "split rows": (257, 512, 800), "tiles": (100, 38408, 96), "one tile": (128, 256, 256), "pairs": (300, 7176, 352), "pair edge": (513, 6416, 544)}
+FORMS = {"split": (77, 1288, 1056), "split rows": (257, 512, 800), "tiles": (100, 38408, 96), "one tile": (128, 256, 256), "pairs": (300, 7176, 352), "pair edge": (513, 6416, 544),
+         "8 parts": (77, 1288, 3232), "8 parts of rows": (257, 512, 4000), "3 parts": (129, 5128, 10272), "3 parts, few rows": (20, 9480, 800),
+         "2 parts, few rows": (31, 15368, 544), "pair of one": (128, 15368, 544)}
 
 
 @pytest.mark.gpu
