@@ -40,6 +40,7 @@ constexpr int NT = 64 + 256;
 // storing the parts of 256 rows about 8 (600 rows and keys of 10 heads in 16.3 us by one CTA, 19.3 by two; 3000 keys in 24.5 by
 // six, 30.2 by three).
 constexpr int LEAST = 4;
+constexpr int MAX_SPLIT = 8; // CTAs of a cluster
 
 template <int HD>
 struct PkSmem {
@@ -220,14 +221,11 @@ __device__ __forceinline__ uint32_t parts_of(int blocks, int least, uint32_t mos
 //            would be nearly empty and, at 1400 clocks for 128 keys, slower than HBM. The warps have the same rows and take
 //            16 keys of each block; their parts, and then the cluster's, are joined in a fixed order.
 //   by rows  short documents: 64 / group query rows a run, the warps' rows are different ones. A CTA is a fraction of the big
-//            kernel's, starts faster, and several fit an SM.
+//            kernel's, starts faster, and two fit an SM: 24 documents of 64 rows and keys and 6 heads of 64 take 5.5 us against
+//            9.1 and 13.5 by keys, of 128 dims 7.0 against 10.2 and 16.4.
 // S (16 x 16 keys) = Q K^T: Q's fragments in registers, K's by ldmatrix; P stays in registers (an MMA's sums are the next
 // one's A fragment); O (16 x HD) += P V, V's fragments by ldmatrix.trans. Keys past a block's end get -infinity and V 0.
 constexpr int FEW_ROWS = 16, FEW_KEYS = 64, FEW_STAGES = 3, FEW_WARPS = 4, FEW_NT = 32 + 32 * FEW_WARPS, FEW_SPLIT = 16;
-// Stacked rows of an average document up to which heads of 64 dims go by rows: 24 documents and 6 heads take 4.6 against 7.7 us
-// at 16 rows, 8.5 against 12.3 at 64, 17.5 against 19.7 at 128 and 29.0 against 24.8 at 192 (behind a prefix of 512 keys 15.5
-// against 26.9 at 16, 38.5 against 36.1 at 128). Heads of 128 dims, four times the work a run, are faster in the big kernel.
-constexpr int SHORT_ROWS = 128;
 constexpr int FEW_LEAST = 16; // blocks that a CTA takes before another one joins it: about 8 us against 7 of starting and joining
 
 template <int HD>
@@ -1000,53 +998,87 @@ void launch(const PackedAttnParams& p, const PkMaps& maps, const PkArgs& a, cuda
         at[0].val.clusterDim.x = unsigned(split);
         c.gridDim = dim3(unsigned(ctas));
     };
-    const long long keys = p.prefix + (p.k_rows - p.prefix) / p.docs; // an average document's
-    // The CTAs of a run's cluster: doubled while there are at most `room` in all and an average document would use half of
-    // them (`least` keys each); a run without the keys for all of them leaves some out.
-    auto split_of = [&](int rows, int room, int least, int most) {
-        const long long runs = std::max<long long>(p.docs, ((long long)p.q_rows + rows - 1) / rows) * p.kv_heads;
-        int split = 1;
-        while (split < most && runs * split * 2 <= room && keys >= (long long)split * least)
-            split *= 2;
-        return split;
+    enum Kernel { BY_KEYS, BY_ROWS, TILES };
+    const int run_rows[3] = {FEW_ROWS / a.group, FEW_ROWS * FEW_WARPS / a.group, 4 * a.unit_rows}; // query rows of a run
+    auto shape = [&](Kernel k) {
+        c.blockDim = dim3(k == TILES ? NT : FEW_NT);
+        c.dynamicSmemBytes = k == TILES ? PkSmem<HD>::TOTAL : FewSmem<HD>::TOTAL;
     };
-    // Documents of a few rows on average (two runs of 16 stacked rows at most), and short ones, go to the kernel for small runs.
-    const long long stacked = (long long)p.q_rows * a.group;
-    if (a.group <= FEW_ROWS && stacked <= 2LL * FEW_ROWS * p.docs) {
-        static std::atomic<uint64_t> opt_in, wide;
-        smem_opt_in(small_runs_kernel<HD, F16, true>, FewSmem<HD>::TOTAL, opt_in);
-        if (!(wide.load() & device_bit())) {
-            H3_CUDA(cudaFuncSetAttribute(small_runs_kernel<HD, F16, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-            wide.fetch_or(device_bit());
-        }
-        const int rows = FEW_ROWS / a.group;
-        c.blockDim = dim3(FEW_NT);
-        c.dynamicSmemBytes = FewSmem<HD>::TOTAL;
-        int split = split_of(rows, 4 * num_sms(), FEW_LEAST * FEW_KEYS, FEW_SPLIT);
-        static ClusterLimits limits; // a cluster of more than eight is the device's to grant
-        if (split > 8 && limits.at_once(small_runs_kernel<HD, F16, true>, c, split) < 1)
-            split = 8;
-        grid(rows, split);
-        H3_CUDA(cudaLaunchKernelEx(&c, small_runs_kernel<HD, F16, true>, maps, a, p.q, p.q_stride));
-        return;
+    auto clusters = [&](Kernel k, int size) { // that the device holds at once
+        static ClusterLimits by_keys, by_rows, tiles;
+        shape(k);
+        return double(k == BY_KEYS   ? by_keys.at_once(small_runs_kernel<HD, F16, true>, c, size)
+                      : k == BY_ROWS ? by_rows.at_once(small_runs_kernel<HD, F16, false>, c, size)
+                                     : tiles.at_once(packed_attention_kernel<HD, F16>, c, size));
+    };
+    static std::atomic<uint64_t> opt_in[3], wide;
+    smem_opt_in(small_runs_kernel<HD, F16, true>, FewSmem<HD>::TOTAL, opt_in[0]);
+    smem_opt_in(small_runs_kernel<HD, F16, false>, FewSmem<HD>::TOTAL, opt_in[1]);
+    smem_opt_in(packed_attention_kernel<HD, F16>, PkSmem<HD>::TOTAL, opt_in[2]);
+    if (!(wide.load() & device_bit())) {
+        H3_CUDA(cudaFuncSetAttribute(small_runs_kernel<HD, F16, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        wide.fetch_or(device_bit());
     }
-    if constexpr (HD == 64)
-        if (stacked <= (long long)SHORT_ROWS * p.docs) {
-            static std::atomic<uint64_t> opt_in;
-            smem_opt_in(small_runs_kernel<HD, F16, false>, FewSmem<HD>::TOTAL, opt_in);
-            grid(FEW_ROWS * FEW_WARPS / a.group, 1);
-            c.blockDim = dim3(FEW_NT);
-            c.dynamicSmemBytes = FewSmem<HD>::TOTAL;
-            H3_CUDA(cudaLaunchKernelEx(&c, small_runs_kernel<HD, F16, false>, maps, a, p.q, p.q_stride));
-            return;
-        }
-    static std::atomic<uint64_t> opt_in;
-    smem_opt_in(packed_attention_kernel<HD, F16>, PkSmem<HD>::TOTAL, opt_in);
-    const int rows = 4 * a.unit_rows;
-    grid(rows, split_of(rows, num_sms(), LEAST * 128, 8));
-    c.blockDim = dim3(NT);
-    c.dynamicSmemBytes = PkSmem<HD>::TOTAL;
-    H3_CUDA(cudaLaunchKernelEx(&c, packed_attention_kernel<HD, F16>, maps, a));
+
+    // The kernel and the CTAs of a run's cluster: the least of what the forms would take, in us, on documents of average length
+    // (the longest: UNEVEN times as many keys). A form takes the waves of its runs, and at least its longest run. The constants
+    // are fits to 1343 calls (1 to 200 documents of 1 to 200 rows on 40 to 6000 keys, even and uneven, four to ten kinds of heads,
+    // each in every form): the form so chosen takes 2.3% longer than the fastest one, in the mean; a rule on rows alone 15%, at
+    // worst 91 us for 12.8 (heads of 64, 8 rows of 8 shared heads on 6000 keys).
+    constexpr double UNEVEN = 1.6;
+    constexpr double KEYS_ALONE = HD == 128 ? 0.55 : 0.38, KEYS_FULL = HD == 128 ? 0.7 : 0.55; // 64 keys of a run: alone, in a full device
+    constexpr double ROWS_BLOCK = HD == 128 ? 2.4 : 1.3;                                       // 64 keys
+    constexpr double TILES_BLOCK = HD == 128 ? 1.1 : 0.9;                                      // 128 keys
+    const double docs = p.docs, keys = p.prefix + (p.k_rows - p.prefix) / docs, stacked = std::ceil(double(p.q_rows) * a.group / docs);
+    auto runs_of = [&](Kernel k) { return docs * p.kv_heads * std::ceil(stacked / (run_rows[k] * a.group)); };
+    const double blocks64 = std::ceil(keys / 64), long64 = std::ceil(blocks64 * (p.docs > 1 ? UNEVEN : 1));
+    const double blocks128 = std::ceil(keys / 128), long128 = std::ceil(blocks128 * (p.docs > 1 ? UNEVEN : 1));
+    auto keys_parts = [&](int split, double blocks) { return std::min<double>(split, std::max(1.0, std::ceil(blocks / FEW_LEAST))); };
+    auto by_keys_us = [&](int split) {
+        const double at_once = clusters(BY_KEYS, split);
+        if (at_once < 1)
+            return HUGE_VAL;
+        const double runs = runs_of(BY_KEYS), w = runs / at_once, waves = std::max(1.0, (w + std::ceil(w)) / 2), used = keys_parts(split, blocks64);
+        const double all = std::ceil(blocks64 / used) * (KEYS_ALONE + (KEYS_FULL - KEYS_ALONE) * std::min(1.0, w)) * waves;
+        const double one = std::ceil(long64 / keys_parts(split, long64)) * KEYS_ALONE;
+        const double launched = (double(p.q_rows) / run_rows[BY_KEYS] + docs) * p.kv_heads * split; // those without work take time too
+        return 6 + 6 * (waves - 1) + std::max(all, one) + (used > 1 ? 2 : 0) + 6 * std::max(0.0, launched - runs * used) / clusters(BY_KEYS, 1);
+    };
+    auto by_rows_us = [&] {
+        const double waves = std::max(1.0, std::ceil(runs_of(BY_ROWS) / clusters(BY_ROWS, 1)));
+        return 2.5 + 4.5 * (waves - 1) + blocks64 * ROWS_BLOCK * std::max(waves, p.docs > 1 ? UNEVEN : 1.0);
+    };
+    auto tiles_parts = [&](int split, double blocks) { return blocks < 2 * LEAST ? 1.0 : std::min<double>(split, std::ceil(blocks / LEAST)); };
+    auto tiles_us = [&](int split) {
+        const double at_once = clusters(TILES, split), used = tiles_parts(split, blocks128);
+        if (at_once < 1)
+            return HUGE_VAL;
+        const double waves = std::max(1.0, std::ceil(runs_of(TILES) / at_once));
+        const double around = 9 + (used > 1 ? 6.5 : 0); // starting, storing, and joining parts
+        return std::max((around + std::ceil(blocks128 / used) * TILES_BLOCK) * waves, around + std::ceil(long128 / tiles_parts(split, long128)) * TILES_BLOCK);
+    };
+    Kernel kernel = TILES;
+    int split = 1;
+    double least = HUGE_VAL;
+    auto consider = [&](Kernel k, int n, double us) {
+        if (us < least)
+            least = us, kernel = k, split = n;
+    };
+    if (a.group <= FEW_ROWS)
+        for (int n = 1; n == 1 || (n <= FEW_SPLIT && n < 2 * keys_parts(FEW_SPLIT, long64)); n *= 2)
+            consider(BY_KEYS, n, by_keys_us(n));
+    consider(BY_ROWS, 1, by_rows_us());
+    for (int n = 1; n <= tiles_parts(MAX_SPLIT, long128); ++n)
+        consider(TILES, n, tiles_us(n));
+
+    grid(run_rows[kernel], split);
+    shape(kernel);
+    if (kernel == BY_KEYS)
+        H3_CUDA(cudaLaunchKernelEx(&c, small_runs_kernel<HD, F16, true>, maps, a, p.q, p.q_stride));
+    else if (kernel == BY_ROWS)
+        H3_CUDA(cudaLaunchKernelEx(&c, small_runs_kernel<HD, F16, false>, maps, a, p.q, p.q_stride));
+    else
+        H3_CUDA(cudaLaunchKernelEx(&c, packed_attention_kernel<HD, F16>, maps, a));
 }
 
 } // namespace

@@ -4,6 +4,7 @@ import ctypes
 import os
 import subprocess
 
+import numpy as np
 import pytest
 import torch
 
@@ -326,3 +327,26 @@ def test_the_attention_half_of_a_block_on_packed_documents_in_4_bits(cuda, f):
     sums = values(A2, rows).abs() @ values(B2, dim).abs().T
     want = before.double() + gate * y
     assert ((x - want).abs() <= gate.abs() * (inner + 4) * 2.0 ** -23 * sums + 2.0 ** -23 * (want.abs() + (gate * y).abs())).all()
+
+
+# documents x (query rows, keys): few and many rows on few and many keys, where one kernel or another, and whole or split runs, are the fastest
+MIXES = [(24, 64, 60), (24, 4, 300), (3, 200, 40), (4, 8, 4000), (3, 64, 6000), (16, 16, 2000), (1, 64, 6000), (60, 20, 300), (3, 600, 1500), (9, 130, 900)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type", list(TYPES))
+@pytest.mark.parametrize("heads,kv,dim", [(6, 6, 64), (3, 3, 128), (8, 2, 128), (16, 1, 64), (20, 1, 128)])
+@pytest.mark.parametrize("docs,rows,keys", MIXES)
+def test_every_kind_of_batch(cuda, type, heads, kv, dim, docs, rows, keys):
+    """Uneven documents around those averages, one of them without keys of its own."""
+    rng = np.random.default_rng(docs + rows + keys)
+    q_start, k_start = (starts(np.maximum(1, rng.uniform(0.3, 1.7, docs) * n).astype(int).tolist(), lead) for n, lead in ((rows, 0), (keys, 70)))
+    if docs > 2:
+        k_start[2] = k_start[1]
+    g = torch.Generator(device=cuda).manual_seed(rows)
+    q, k, v = (torch.randn(n, h, dim, generator=g, device=cuda).to(TYPES[type][0]) for n, h in ((q_start[-1], heads), (k_start[-1], kv), (k_start[-1], kv)))
+    out = torch.full_like(q, 7.0)
+    before = out.clone()
+    at_q, at_k = (torch.tensor(s, dtype=torch.int32, device=cuda) for s in (q_start, k_start))
+    call(q, k, v, out, at_q, at_k, 70)
+    compare(out, *expected(q, k, v, q_start, k_start, 70, dim ** -0.5, before))
