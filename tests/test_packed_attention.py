@@ -3,6 +3,7 @@ see: refusals on the CPU, the kernel on a B200, alone and in the chain of 4-bit 
 import ctypes
 import os
 import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -350,3 +351,32 @@ def test_every_kind_of_batch(cuda, type, heads, kv, dim, docs, rows, keys):
     at_q, at_k = (torch.tensor(s, dtype=torch.int32, device=cuda) for s in (q_start, k_start))
     call(q, k, v, out, at_q, at_k, 70)
     compare(out, *expected(q, k, v, q_start, k_start, 70, dim ** -0.5, before))
+
+
+FIRST = """
+import ctypes, sys, torch
+import h3b200 as H
+sys.path.insert(0, {tests!r})
+import test_packed_attention as T
+dev = torch.device("cuda")
+q, k, v = (torch.randn(n, 2, 128, device=dev).bfloat16() for n in ({rows}, {keys}, {keys}))
+out, again = torch.zeros_like(q), torch.zeros_like(q)
+at_q, at_k = (torch.tensor([0, n], dtype=torch.int32, device=dev) for n in ({rows}, {keys}))
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    T.call(q, k, v, out, at_q, at_k, 0, check=False)
+graph.replay()
+torch.cuda.synchronize()
+T.call(q, k, v, again, at_q, at_k, 0)
+assert torch.equal(out, again) and out.abs().sum() > 0
+"""
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,keys", [(1, 9000), (40, 50), (900, 900)])
+def test_the_first_call_of_a_process_may_be_captured(cuda, rows, keys):
+    here = os.path.dirname(os.path.abspath(__file__))
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([os.path.join(here, "..", "mako-video_b200"), os.path.join(here, ".."), os.environ.get("PYTHONPATH", "")]))
+    r = subprocess.run([sys.executable, "-c", FIRST.format(tests=here, rows=rows, keys=keys)], env=env, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
