@@ -39,6 +39,16 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b)
     return d;
 }
 
+__device__ __forceinline__ float2 mul2_rz(float2 a, float2 b)
+{
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+        "mul.rz.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
 // Sixteen consecutive values of a row, as loaded.
 template <Elem T>
 struct Run {
@@ -159,19 +169,40 @@ __device__ __forceinline__ uint2 encode(const Run<T>& x, uint32_t most, float rg
         for (int i = 0; i < 8; ++i)
             q[i] = mul2(x.pair(i), inv);
     } else {
-        // A quotient rounded to nearest from the divisor's rounded reciprocal: one residual step (Markstein). For the six here,
-        // and for the codes: x / c has to be exact where it lies on the border of two codes, where ties go by the code.
+        // A quotient rounded to nearest from the divisor's rounded reciprocal: one residual step (Markstein).
         const float m = __uint_as_float(most) * rg;
         const float m6 = m * (1.f / 6.f);
         byte = to_e4m3(fmaf(fmaf(-m6, 6.f, m), 1.f / 6.f, m6));
         const float c = from_e4m3(byte);
         const float inv = c > 0.f ? reciprocal_e4m3(c) : 0.f;
-        const float2 rg2 = make_float2(rg, rg), inv2 = make_float2(inv, inv), nc2 = make_float2(-c, -c);
+        if constexpr (T == Elem::f32) {
+            // the same for the codes: fp32 values come as near to the border of two codes as the quotient's rounding
+            const float2 rg2 = make_float2(rg, rg), inv2 = make_float2(inv, inv), nc2 = make_float2(-c, -c);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float2 s = mul2(x.pair(i), rg2);
-            const float2 f = mul2(s, inv2);
-            q[i] = fma2(fma2(f, nc2, s), inv2, f);
+            for (int i = 0; i < 8; ++i) {
+                const float2 s = mul2(x.pair(i), rg2);
+                const float2 f = mul2(s, inv2);
+                q[i] = fma2(fma2(f, nc2, s), inv2, f);
+            }
+        } else {
+            // x / c has to be exact where it lies on the border t of two codes, where ties go by the code, and on its side of it
+            // elsewhere. x = t c: the reciprocal of an e4m3 number rounded to nearest is 1 / c (1 + d) with 0 <= d < 2^-24 (so
+            // for all eight significands), and t (1 + d) rounded towards zero is t. Else x / c is 2^-13 or more from t (x has 11 bits at
+            // most, t c seven), far more than d and the rounding. (33024 x 13824 in 196 us so, 230 by the residual.)
+            float k = inv * rg;
+            if (rg > 0x1p118f) { // rows below 2^-107: k could overflow
+                k = inv;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    q[i] = mul2(x.pair(i), make_float2(rg, rg));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    q[i] = x.pair(i);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                q[i] = mul2_rz(q[i], make_float2(k, k));
         }
     }
     return make_uint2(e2m1x8(q[0], q[1], q[2], q[3]), e2m1x8(q[4], q[5], q[6], q[7]));
@@ -226,7 +257,7 @@ constexpr int QUANT_THREADS = 512; // of a CTA at most
 
 // blockDim.x = 32 x the warps of a row (RUNS runs a thread; a row of more runs than that is read twice instead of kept), or,
 // for SHORT rows of one warp, of as many rows.
-// (64 registers a thread: 33024 x 5120 in 88 us for nv and 67 for mx; unbounded, with 72, 98 and 70.)
+// (64 registers a thread: 33024 x 5120 in 67 us for mx; unbounded, with 72, 70.)
 template <Elem T, Fp4 F, bool SHORT>
 __global__ void __launch_bounds__(QUANT_THREADS, 2) quant_fp4_kernel(const void* x, int64_t ldx, int rows, int K, bool wide, uint8_t* codes,
                                                                   uint8_t* scales, float* row_scale)
@@ -295,12 +326,13 @@ __global__ void __launch_bounds__(QUANT_THREADS, 2) quant_fp4_kernel(const void*
     }
 }
 
-// Long nv rows of 16-bit values: few CTAs of that many threads fit an SM, and all of them wait for a row's last value before
-// they go on. So CTAs stay and walk rows, which bulk copies bring into shared memory ahead of them: 33024 x 13824 in 230 us
-// against 270, x 8224 in 146 against 166; at 5120 the two take the same, below it this one loses.
-constexpr int RING = 3; // rows
+// Many nv rows of 16-bit values: all threads of a row wait for its last value before they go on, and few rows fit an SM's
+// registers. So CTAs walk rows, which bulk copies bring into shared memory one ahead of them, and there are up to four times
+// as many CTAs as an SM holds, at different places in their rows: 33024 x 5120 in 69 us (6.3 TB/s) against 84 by the kernel
+// above, x 2048 in 31 against 33, x 13824 in 200 against 270. (A ring of three rows: 73, 33, 215; as many CTAs as fit: 81 at 5120.)
+constexpr int RING = 2; // rows
 template <Elem T>
-__global__ void __launch_bounds__(QUANT_THREADS, 2) quant_long_rows_kernel(const void* x, int64_t ldx, int rows, int K, uint8_t* codes, uint8_t* scales,
+__global__ void __launch_bounds__(QUANT_THREADS, 2) quant_many_rows_kernel(const void* x, int64_t ldx, int rows, int K, uint8_t* codes, uint8_t* scales,
                                                                         float* row_scale)
 {
     static_assert(T != Elem::f32);
@@ -435,11 +467,14 @@ void quant(const void* x, int64_t ldx, int rows, int K, void* codes, void* scale
     auto* sc = static_cast<uint8_t*>(scales);
     const int warps = (runs + 32 * QUANT_RUNS - 1) / (32 * QUANT_RUNS);
     if constexpr (F == Fp4::nv && T != Elem::f32) {
-        const int threads = 32 * warps, ctas = num_sms() * std::max(1, 1024 / threads); // with 64 registers a thread
-        if (warps > 8 && threads <= QUANT_THREADS && all_rows >= 2 * ctas) {
+        const int threads = 32 * warps, held = num_sms() * std::max(1, std::min(2048 / threads, 220000 / (RING * K * 2 + 1200)));
+        // four rows a CTA at least, and then more CTAs: 4128 x 13824 takes 32 us by two CTAs a place and 37 by four, 4128 x 2048, of
+        // one row a CTA, 8.4 against 6.8 by the other kernel
+        if (warps > 1 && threads <= QUANT_THREADS && all_rows >= 4 * held) {
+            const int ctas = held * std::min(4, all_rows / (4 * held));
             static std::atomic<uint64_t> opt_in;
-            smem_opt_in(quant_long_rows_kernel<T>, RING * 32 * QUANT_RUNS * QUANT_THREADS, opt_in);
-            quant_long_rows_kernel<T><<<ctas, threads, RING * K * 2, s>>>(x, ldx, rows, K, c, sc, row_scale);
+            smem_opt_in(quant_many_rows_kernel<T>, RING * 32 * QUANT_RUNS * QUANT_THREADS, opt_in);
+            quant_many_rows_kernel<T><<<ctas, threads, RING * K * 2, s>>>(x, ldx, rows, K, c, sc, row_scale);
             H3_CUDA(cudaGetLastError());
             return;
         }

@@ -172,6 +172,13 @@ def test_quantise_many_long_rows_bit_exact(cuda, kind, type, rows, K, ld):
     check_quantise(cuda, F4.NV, kind, type, rows, K, ld)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,type,rows,K,ld", [("normal", "bf16", 1801, 16384, 16384), ("wide", "f16", 19001, 1056, 1064), ("wide", "bf16", 5950, 5120, 5128)])
+def test_quantise_many_rows_bit_exact(cuda, kind, type, rows, K, ld):
+    """Enough rows that CTAs walk several."""
+    check_quantise(cuda, F4.NV, kind, type, rows, K, ld)
+
+
 def check_quantise(cuda, f, kind, type, rows, K, ld):
     dtype = TYPES[type][0]
     x = torch.from_numpy(rows_like(rows, ld, rows + K, kind)).clamp(-3e38, 3e38).to(dtype)
@@ -195,6 +202,31 @@ def check_quantise(cuda, f, kind, type, rows, K, ld):
         near = (np.abs(np.abs(q)[..., None] - borders) <= 2.0 ** -23 * borders).any(-1)
         differ &= ~near
     assert not differ.any(), (np.argwhere(differ)[:5], got[differ][:5], want_codes[differ][:5], q[differ][:5])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type,power", [("bf16", n) for n in (-126, -120, -118, -107, 0, 100, 116)] + [("f16", n) for n in (-12, 0, 4)])
+def test_quantise_on_and_beside_every_border_of_every_scale(cuda, type, power):
+    """Blocks of every e4m3 scale c with +-t c for the borders t between codes, exact and one step to either side; row scales 2^power."""
+    dtype = TYPES[type][0]
+    scales = [c for c in F4.e4m3_values().tolist() if 0 < c <= 320]
+    borders = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
+    blocks = [np.concatenate([[6 * c], borders * c, -borders * c, [0.0]]) for c in scales]
+    x = np.concatenate([[2047.0] + [1.0] * 15] + blocks + [np.zeros(16)] * ((len(blocks) + 1) % 2))
+    x = torch.from_numpy(np.stack([x] * 3) * 2.0 ** power).to(dtype)
+    bits = x.view(torch.int16)
+    inner = torch.ones(x.shape[1], dtype=torch.bool)
+    inner[::16] = False  # the blocks' largest stay
+    inner &= x[0] != 0
+    bits[1, inner] += 1
+    bits[2, inner] -= 1
+    got_codes, got_tiles, row = gpu_quantise(x.to(cuda), F4.NV)
+    codes, bytes_, want_row, _ = F4.quantise(x.double().numpy(), F4.NV)
+    packed, tiles = F4.pack(codes, bytes_)
+    np.testing.assert_array_equal(got_tiles.cpu().numpy(), tiles)
+    np.testing.assert_array_equal(row.cpu().numpy().astype(np.float64), want_row)
+    got, _ = F4.unpack(got_codes.cpu().numpy().reshape(x.shape[0], -1), tiles, F4.NV)
+    np.testing.assert_array_equal(np.where(got == 8, 0, got), codes)
 
 
 @pytest.mark.gpu
