@@ -179,6 +179,20 @@ def test_quantise_many_rows_bit_exact(cuda, kind, type, rows, K, ld):
     check_quantise(cuda, F4.NV, kind, type, rows, K, ld)
 
 
+@pytest.mark.gpu
+def test_rows_in_one_call_are_those_of_many_calls(cuda):
+    """Many rows (walked by CTAs) against 2048 at a time (a CTA each), infinities and NaNs among them, bit for bit."""
+    rows, K = 19000, 1056
+    x = torch.randn(rows, K, device=cuda).bfloat16()
+    x[::7] *= 2.0 ** -120
+    x[5, 1055], x[4000, 0], x[18999, 7], x[130] = float("nan"), float("inf"), float("-inf"), 0
+    codes, tiles, row = gpu_quantise(x, F4.NV)
+    parts = [gpu_quantise(x[i:i + 2048], F4.NV) for i in range(0, rows, 2048)]
+    for whole, n in ((codes, 0), (tiles, 1), (row, 2)):
+        assert torch.equal(whole.view(torch.uint8), torch.cat([part[n] for part in parts]).view(torch.uint8))
+    assert torch.isnan(row).nonzero().flatten().tolist() == [5, 4000, 18999]
+
+
 def check_quantise(cuda, f, kind, type, rows, K, ld):
     dtype = TYPES[type][0]
     x = torch.from_numpy(rows_like(rows, ld, rows + K, kind)).clamp(-3e38, 3e38).to(dtype)
