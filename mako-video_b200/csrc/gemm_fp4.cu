@@ -545,7 +545,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         if (elected)
             commit<PAIR>(drain);
         __syncwarp();
-        mbar_wait(drain, 0);
+        mbar_wait_landed(drain, 0);
     } else if (warp >= 2) {
         // ---------------------------------------------------------------------------------------- epilogue
         const int quarter = warp & 3, half = (warp - 2) >> 2; // its 32 TMEM lanes, its half of the columns
@@ -613,8 +613,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if constexpr (PAIR)
+    if constexpr (PAIR) {
+        // The closing commit arrives in both CTAs, each of which has to see it before its shared memory may go: that it has
+        // arrived in the first says nothing of the second. (Here, after the tiles, so that the wait's bound is not theirs.)
+        if (part == 1 && warp == 1)
+            mbar_wait_landed(drain, 0);
         cluster_sync(); // no MMA of the pair is under way
+    }
     if (warp == 1) {
         tc_fence_after();
         tmem_free<PAIR>(tmem);

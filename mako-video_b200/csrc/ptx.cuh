@@ -80,6 +80,21 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, long l
     }
 }
 
+// mbar_wait for what the hardware still writes into this CTA's shared or tensor memory (its copies under way, commits that
+// arrive on its barriers), before the CTA exits: bounded by time alone, since neither stops at a failure elsewhere.
+__device__ __forceinline__ bool mbar_wait_landed(uint64_t* bar, uint32_t parity, long long budget = 4000000000ll)
+{
+    if (mbar_try_wait(bar, parity))
+        return true;
+    const long long t0 = clock64();
+    while (!mbar_try_wait(bar, parity))
+        if (clock64() - t0 > budget) {
+            record_error(kErrWaitTimeout);
+            return false;
+        }
+    return true;
+}
+
 // ------------------------------------------------------------------------------------------------------ TMA
 __device__ __forceinline__ void tma_prefetch_desc(const void* tmap)
 {

@@ -535,3 +535,32 @@ def test_product_without_bias_or_row_scales_and_one_row_of_any_pitch(cuda):
     want = (A[3] / A[2].double()[:, None]) @ (B[3] / B[2].double()[:, None]).T
     tol = K * 2.0 ** -23 * ((A[3] / A[2].double()[:, None]).abs() @ (B[3] / B[2].double()[:, None]).abs().T)
     assert ((out[:N] - want[0]).abs() <= tol[0]).all() and (out[N:] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f", FORMATS)
+def test_pairs_that_follow_one_another_at_once(cuda, f):
+    """Products of one and of a few pairs of CTAs, whose clusters end while others start on the same SMs, queued on two streams without
+    a wait: every result is bit for bit that of the call alone."""
+    calls = []
+    for M, N, K in ((128, 15368, 544), (300, 776, 352), (513, 264, 96), (130, 4104, 256)):
+        A, B = operand(M, K, f, M, cuda), operand(N, K, f, N, cuda, 0.1)
+        out = [torch.zeros(M, N, device=cuda, dtype=torch.bfloat16) for _ in range(2)]
+        args = [H.h3k_gemm_args(M=M, N=N, K=K, a_scale=p(A[2]), b_scale=p(B[2]), out=p(o), ldo=N) for o in out]
+        calls.append((A, B, out, args))
+    go = lambda A, B, args: H.check(H.lib().h3k_gemm_fp4(p(A[0]), p(A[1]), p(B[0]), p(B[1]), f, ctypes.byref(args), H.EPI_BF16, stream()))
+    want = []
+    for A, B, out, args in calls:
+        go(A, B, args[0])
+        sync()
+        want.append(out[0].clone())
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    for i in range(200):
+        for s, side in enumerate(sides):
+            with torch.cuda.stream(side):
+                A, B, out, args = calls[(i + 2 * s) % len(calls)]
+                go(A, B, args[s])
+    torch.cuda.synchronize()
+    sync()
+    for w, (A, B, out, args) in zip(want, calls):
+        assert torch.equal(out[0], w) and torch.equal(out[1], w)
