@@ -362,8 +362,7 @@ __global__ void __launch_bounds__(QUANT_THREADS, 2) quant_many_rows_kernel(const
     int turn = 0;
     for (int64_t r = blockIdx.x; r < all_rows; r += gridDim.x, ++turn) {
         const bool in = r < rows;
-        if (in && !mbar_wait(&full[turn % RING], (turn / RING) & 1))
-            return; // (the device error is set; this CTA's copies have had seconds to land)
+        const bool late = in && !mbar_wait(&full[turn % RING], (turn / RING) & 1); // (the device error is set: see below)
         const uint4* row = reinterpret_cast<const uint4*>(ring + (turn % RING) * bytes);
         Run<T> keep[RUNS];
         uint32_t most[RUNS], all = 0;
@@ -380,13 +379,25 @@ __global__ void __launch_bounds__(QUANT_THREADS, 2) quant_many_rows_kernel(const
                 all = max(all, most[i]);
             }
         }
-        all = __reduce_max_sync(0xffffffffu, all);
+        // A wait that gave up, of whichever thread, ends the CTA: all of it, so that no warp waits at the barrier for one that has
+        // left, and not before its copies have landed. (Another kernel's failure ends waits long before their time, so that
+        // nothing else says that they have.) It goes with the maxima, as what no magnitude is: a
+        // barrier that votes costs 2 to 5% of the call.
+        constexpr uint32_t LATE = 0xffffffffu;
+        all = __reduce_max_sync(0xffffffffu, late ? LATE : all);
         if (lane_id() == 0)
             red[turn & 1][warp_id()] = all;
         __syncthreads(); // the row is in registers, and the warps' maxima are there
-        if (t == 0)
+        if (t == 0 && !late)
             fetch(r + int64_t(RING) * gridDim.x, turn);
         all = __reduce_max_sync(0xffffffffu, lane_id() < int(blockDim.x) / 32 ? red[turn & 1][lane_id()] : 0);
+        if (all == LATE) {
+            if (t == 0)
+                for (int i = late ? 0 : 1, end = i + RING; i < end; ++i) // this thread's copies that it has not seen land
+                    if (r + int64_t(i) * gridDim.x < rows)
+                        mbar_wait_landed(&full[(turn + i) % RING], ((turn + i) / RING) & 1, 100000000ll);
+            return;
+        }
         float scale;
         const float rg = row_scale_of(all, scale);
         if (in && t == 0)
