@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(FEW_NT, 2) small_runs_kernel(const __grid_cons
             }
             // Every load lands before the CTA can exit.
             for (int i = max(0, j - FEW_STAGES); i < j; ++i)
-                mbar_wait(&full[i % FEW_STAGES], (i / FEW_STAGES) & 1);
+                mbar_wait_landed(&full[i % FEW_STAGES], (i / FEW_STAGES) & 1);
         }
     } else {
         uint32_t qf[HD / 16][4];
@@ -647,11 +647,11 @@ __device__ __forceinline__ void attend(const PkMaps& maps, const PkArgs& p, cons
         }
         // Loads that no one waited for (a pipeline that gave up) land before the CTA can exit.
         if (nkv > 0)
-            mbar_wait(q_full, 0);
+            mbar_wait_landed(q_full, 0);
         for (int j = max(0, jk - KST); j < jk; ++j)
-            mbar_wait(&k_full[j % KST], (j / KST) & 1);
+            mbar_wait_landed(&k_full[j % KST], (j / KST) & 1);
         for (int j = max(0, jv - vst); j < jv; ++j)
-            mbar_wait(&v_full[j % vst], (j / vst) & 1);
+            mbar_wait_landed(&v_full[j % vst], (j / vst) & 1);
     } else if (warp == 1) {
         // ------------------------------------------------------------------------------------------ MMA
         // The warp stays converged and one lane issues, so that descriptors are made in uniform registers.
@@ -709,7 +709,7 @@ __device__ __forceinline__ void attend(const PkMaps& maps, const PkArgs& p, cons
         if (elected)
             mma_commit(drain);
         __syncwarp();
-        mbar_wait(drain, 0);
+        mbar_wait_landed(drain, 0);
     } else if (warp >= 2) {
         // -------------------------------------------------------------------------------------- softmax
         const int t = (warp - 2) / 4;

@@ -502,10 +502,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 }
             }
         }
-        // Wait for the loads still in flight to land before the CTA can exit.
-        if (ok)
-            for (uint32_t j = it >= STAGES ? it - STAGES : 0; j < it; ++j)
-                mbar_wait(&empty[j % STAGES], (j / STAGES) & 1);
+        // Wait for the loads still in flight to land before the CTA can exit: until the MMAs have read them, or, when a wait gave up and
+        // no MMA may follow, for as many times the time that a load takes.
+        for (uint32_t j = it >= STAGES ? it - STAGES : 0; j < it; ++j)
+            mbar_wait_landed(&empty[j % STAGES], (j / STAGES) & 1, ok ? 4000000000ll : 100000000ll);
     } else if (warp == 1 && (!PAIR || part == 0)) {
         // ------------------------------------------------------------------------------------- MMA issuer
         uint32_t elected;
