@@ -328,7 +328,8 @@ int h3k_heads(const float* x, int64_t ldx, int32_t rows, const float* W, const f
  * Returns H3_ERR_DEVICE with the device error, as a step whose pipeline wait ran out does; the context stays usable
  * and the error word is cleared. */
 int h3k_wait_selftest(uint64_t budget_cycles, void* stream);
-/* Waits for `stream` and reports a device-side failure (bounded wait ran out) as H3_ERR_DEVICE. */
+/* Waits for `stream` and reports a device-side failure (bounded wait ran out; bad starts in a call of
+ * h3k_attention_packed without a status word), of whichever stream of the device, once as H3_ERR_DEVICE. */
 int h3k_check(void* stream);
 
 /* ------------------------------------------------------------------------------------------ video VAE decoder
@@ -436,9 +437,12 @@ typedef struct h3k_packed_args {
     int32_t q_rows, k_rows;                           /* rows of q and out, of k and v */
     int32_t docs, prefix;
     const int32_t* q_start; /* [docs + 1], ascending, in device memory, read when the work runs (a replayed graph sees */
-    const int32_t* k_start; /* new values): starts out of order or out of the rows are a device error (h3k_check), after */
-                            /* which what the call wrote is not to be used; nothing outside the rows is touched */
+    const int32_t* k_start; /* new values): after starts out of order or out of the rows, which `status` or h3k_check tells, */
+                            /* what the call wrote is not to be used; nothing outside the rows is touched */
     float scale;            /* 0: 1 / sqrt(head_dim) */
+    int32_t* status;        /* a word that the GPU can write: 1 or 0, written by every run, whether the starts were bad. NULL: */
+                            /* bad starts are a device error that the next h3k_check on the device reports, whoever calls it */
+                            /* (no step or decode does, nor fails for it); where several callers share a device, give a word */
 } h3k_packed_args;
 /* out overlaps none of the others. Queued on `stream`, no scratch and no synchronisation; may be captured into a graph. */
 int h3k_attention_packed(const h3k_packed_args* args, void* stream);

@@ -62,6 +62,7 @@ struct PkArgs {
     int64_t out_stride;
     const int32_t* q_start;
     const int32_t* k_start;
+    int32_t* status;
     int q_rows, k_rows, kv_heads, docs, prefix, group, unit_rows; // unit_rows: query rows in a 64-row unit, 64 / group
     float sl2;                                          // scale log2(e)
 };
@@ -191,13 +192,21 @@ __device__ __forceinline__ Run run_of(const PkArgs& p, int slot, int run_rows)
     return r;
 }
 
-// The starts ascend within the tensors; what else they say is a device error, and such documents are left out.
+// The starts ascend within the tensors; what else they say is told to the caller, and such documents are left out. One CTA, all
+// of its threads.
 __device__ __forceinline__ void check_starts(const PkArgs& p, int threads)
 {
+    bool bad = false;
     for (int d = threadIdx.x; d <= p.docs; d += threads) {
         const int a = p.q_start[d], b = p.k_start[d];
-        if (a < 0 || a > p.q_rows || b < 0 || b > p.k_rows || (d > 0 && (a < p.q_start[d - 1] || b < p.k_start[d - 1])))
-            record_error(kErrBadShape);
+        bad |= a < 0 || a > p.q_rows || b < 0 || b > p.k_rows || (d > 0 && (a < p.q_start[d - 1] || b < p.k_start[d - 1]));
+    }
+    bad = __syncthreads_or(bad);
+    if (threadIdx.x == 0) {
+        if (p.status)
+            *p.status = bad;
+        else if (bad)
+            record_data_error(kDataStarts);
     }
 }
 
@@ -1092,7 +1101,7 @@ void attention_packed(const PackedAttnParams& p, cudaStream_t s)
     maps.k = p.k_rows > 0 ? rows_map(p.k, p.f16, p.kv_heads, p.k_rows, p.k_stride, p.head_dim, 1, 64) : maps.q;
     maps.v = p.k_rows > 0 ? rows_map(p.v, p.f16, p.kv_heads, p.k_rows, p.v_stride, p.head_dim, 1, 64) : maps.q;
     PkArgs a{};
-    a.out = p.out, a.out_stride = p.out_stride, a.q_start = p.q_start, a.k_start = p.k_start, a.q_rows = p.q_rows, a.k_rows = p.k_rows;
+    a.out = p.out, a.out_stride = p.out_stride, a.q_start = p.q_start, a.k_start = p.k_start, a.status = p.status, a.q_rows = p.q_rows, a.k_rows = p.k_rows;
     a.kv_heads = p.kv_heads, a.docs = p.docs, a.prefix = p.prefix, a.group = group, a.unit_rows = unit_rows;
     a.sl2 = float(double(p.scale) * 1.4426950408889634);
     if (p.head_dim == 128)

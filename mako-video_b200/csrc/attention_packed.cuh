@@ -22,6 +22,7 @@ struct PackedAttnParams {
     const int32_t* q_start = nullptr;
     const int32_t* k_start = nullptr;
     float scale = 0.f;
+    int32_t* status = nullptr; // 1 where the starts are out of order or out of the rows, else 0 (null: a data error)
 };
 
 void attention_packed(const PackedAttnParams& p, cudaStream_t s);

@@ -848,8 +848,12 @@ int h3k_check(void* stream)
 {
     return guarded([&] {
         H3_CUDA(cudaStreamSynchronize(st(stream)));
-        if (const uint32_t e = h3::take_device_error(st(stream)))
-            throw DeviceError("device error " + std::to_string(e) + ": a kernel's bounded wait ran out");
+        const uint32_t e = h3::take_device_error(st(stream)), data = h3::take_data_error(st(stream));
+        const std::string starts = "h3k_attention_packed found starts out of order or out of the rows";
+        if (e)
+            throw DeviceError("device error " + std::to_string(e) + ": a kernel's bounded wait ran out" + (data ? "; " + starts : ""));
+        if (data)
+            throw DeviceError(starts);
     });
 }
 

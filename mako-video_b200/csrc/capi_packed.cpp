@@ -179,8 +179,14 @@ int h3k_attention_packed(const h3k_packed_args* a, void* stream)
         need(a->q_rows >= 0 && a->k_rows >= 0 && a->docs >= 0, call, "a negative number of rows or documents");
         need(a->prefix >= 0 && a->prefix <= a->k_rows, call, "the prefix must lie in the key rows");
         need(a->scale >= 0.f && std::isfinite(a->scale), call, "the scale must be positive (0: 1 / sqrt(head_dim))");
-        if (a->q_rows == 0 || a->docs == 0)
+        need(aligned(a->status, 4), call, "a pointer is not aligned");
+        if (a->q_rows == 0 || a->docs == 0) {
+            if (a->status) {
+                device_only(call, {a->status});
+                H3_CUDA(cudaMemsetAsync(a->status, 0, sizeof(int32_t), static_cast<cudaStream_t>(stream)));
+            }
             return;
+        }
         need(a->q && a->out && a->q_start && a->k_start && (a->k_rows == 0 || (a->k && a->v)), call, "null argument");
         need(aligned(a->q, 16) && aligned(a->k, 16) && aligned(a->v, 16) && aligned(a->out, 16) && aligned(a->q_start, 4) && aligned(a->k_start, 4),
              call, "a pointer is not aligned");
@@ -189,11 +195,12 @@ int h3k_attention_packed(const h3k_packed_args* a, void* stream)
         need(rows_ok(a->q_rows, a->q_stride, q_width) && rows_ok(a->q_rows, a->out_stride, q_width) && rows_ok(a->k_rows, a->k_stride, k_width) &&
                  rows_ok(a->k_rows, a->v_stride, k_width),
              call, "rows must not overlap and be 16 bytes aligned");
-        device_only(call, {a->q, a->k, a->v, a->out, a->q_start, a->k_start});
+        device_only(call, {a->q, a->k, a->v, a->out, a->q_start, a->k_start, a->status});
         h3::PackedAttnParams p;
         p.q = a->q, p.k = a->k, p.v = a->v, p.out = a->out, p.q_stride = a->q_stride, p.k_stride = a->k_stride, p.v_stride = a->v_stride;
         p.out_stride = a->out_stride, p.f16 = a->type == H3K_F16, p.heads = a->heads, p.kv_heads = a->kv_heads, p.head_dim = a->head_dim;
         p.q_rows = a->q_rows, p.k_rows = a->k_rows, p.docs = a->docs, p.prefix = a->prefix, p.q_start = a->q_start, p.k_start = a->k_start;
+        p.status = a->status;
         p.scale = a->scale > 0.f ? a->scale : 1.f / std::sqrt(float(a->head_dim));
         h3::attention_packed(p, static_cast<cudaStream_t>(stream));
     });

@@ -7,6 +7,7 @@
 namespace h3 {
 
 __device__ uint32_t g_device_error = 0;
+__device__ uint32_t g_data_error = 0;
 
 namespace {
 
@@ -55,15 +56,23 @@ CUtensorMap make_tmap(CUtensorMapDataType type, int rank, const void* base, cons
     return m;
 }
 
-uint32_t take_device_error(cudaStream_t s)
+namespace {
+
+template <class Word>
+uint32_t take_word(const Word& word, cudaStream_t s)
 {
     uint32_t v = 0, zero = 0;
-    H3_CUDA(cudaMemcpyFromSymbolAsync(&v, g_device_error, sizeof(v), 0, cudaMemcpyDeviceToHost, s));
+    H3_CUDA(cudaMemcpyFromSymbolAsync(&v, word, sizeof(v), 0, cudaMemcpyDeviceToHost, s));
     H3_CUDA(cudaStreamSynchronize(s));
     if (v)
-        H3_CUDA(cudaMemcpyToSymbolAsync(g_device_error, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s));
+        H3_CUDA(cudaMemcpyToSymbolAsync(word, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s));
     return v;
 }
+
+} // namespace
+
+uint32_t take_device_error(cudaStream_t s) { return take_word(g_device_error, s); }
+uint32_t take_data_error(cudaStream_t s) { return take_word(g_data_error, s); }
 
 bool device_accessible(const void* p)
 {

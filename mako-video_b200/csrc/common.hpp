@@ -28,6 +28,8 @@ CUtensorMap make_tmap(CUtensorMapDataType type, int rank, const void* base, cons
 
 // Reads and clears the device error word (nonzero: a kernel's bounded wait ran out or a shape check failed).
 uint32_t take_device_error(cudaStream_t s);
+// The same for the word of what kernels found wrong in callers' data (h3k_check alone).
+uint32_t take_data_error(cudaStream_t s);
 
 int num_sms();
 

@@ -18,6 +18,16 @@ enum DeviceError : uint32_t {
     kErrBadShape = 2,        // a kernel was launched with a shape its preconditions exclude
 };
 
+// What kernels found wrong in a caller's data, in a word of its own: no kernel has failed, so no wait ends early for it and no
+// step reports it; only h3k_check reads and clears it.
+extern __device__ uint32_t g_data_error;
+
+enum DataError : uint32_t {
+    kDataStarts = 1, // documents' starts out of order or out of the rows
+};
+
+__device__ __forceinline__ void record_data_error(uint32_t code) { atomicCAS(&g_data_error, 0u, code); }
+
 __device__ __forceinline__ void record_error(uint32_t code) { atomicCAS(&g_device_error, 0u, code); }
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p)

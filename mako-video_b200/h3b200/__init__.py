@@ -89,7 +89,8 @@ class h3k_packed_args(ctypes.Structure):
                 ("q_stride", ctypes.c_int64), ("k_stride", ctypes.c_int64), ("v_stride", ctypes.c_int64), ("out_stride", ctypes.c_int64),
                 ("type", ctypes.c_int32), ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
                 ("q_rows", ctypes.c_int32), ("k_rows", ctypes.c_int32), ("docs", ctypes.c_int32), ("prefix", ctypes.c_int32),
-                ("q_start", ctypes.c_void_p), ("k_start", ctypes.c_void_p), ("scale", ctypes.c_float)]
+                ("q_start", ctypes.c_void_p), ("k_start", ctypes.c_void_p), ("scale", ctypes.c_float),
+                ("status", ctypes.c_void_p)]
 
 
 class h3k_cube_grid(ctypes.Structure):

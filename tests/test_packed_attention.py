@@ -380,3 +380,86 @@ def test_the_first_call_of_a_process_may_be_captured(cuda, rows, keys):
     env = dict(os.environ, PYTHONPATH=os.pathsep.join([os.path.join(here, "..", "mako-video_b200"), os.path.join(here, ".."), os.environ.get("PYTHONPATH", "")]))
     r = subprocess.run([sys.executable, "-c", FIRST.format(tests=here, rows=rows, keys=keys)], env=env, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+# ------------------------------------------------------------------------- who hears of starts that are not in order
+
+def test_refuses_a_status_word_that_is_not_aligned():
+    a = H.h3k_packed_args(**(GOOD | dict(status=BASE + 2)))
+    assert H.lib().h3k_attention_packed(ctypes.byref(a), None) == H.H3_ERR_ARG
+    assert "aligned" in H.lib().h3_last_error().decode()
+
+
+def queue(q_start, k_start, status=None, rows=20):
+    """A call on `rows` rows of 2 heads of 64, not waited for; what it uses is returned, to be kept."""
+    q, k, v = (torch.randn(rows, 2, 64, device="cuda").half() for _ in range(3))
+    out = torch.zeros_like(q)
+    at = [torch.tensor(s, dtype=torch.int32, device="cuda") if isinstance(s, list) else s for s in (q_start, k_start)]
+    a = H.h3k_packed_args(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(), q_stride=128, k_stride=128, v_stride=128, out_stride=128, type=H.F16,
+                          heads=2, kv_heads=2, head_dim=64, q_rows=rows, k_rows=rows, docs=at[0].numel() - 1, q_start=at[0].data_ptr(), k_start=at[1].data_ptr(),
+                          **({} if status is None else dict(status=status.data_ptr())))
+    H.check(H.lib().h3k_attention_packed(ctypes.byref(a), stream()))
+    return q, k, v, out, at
+
+
+BAD, FINE = [0, 10, 5, 20], [0, 10, 15, 20]
+
+
+@pytest.mark.gpu
+def test_a_step_beside_a_call_with_bad_starts_is_not_told_of_them(cuda):
+    """The steps and decodes of others on the device end well, and the caller still hears of the starts."""
+    from test_step_gpu import MINI, MINI_LAYOUT, inputs
+    lay, text, video, audio = inputs(MINI_LAYOUT, MINI)
+    m = H.Model(MINI, seed=1)
+    m.begin(text, lay)
+    want = m.step(video, audio, 0.7, 0.4)
+    keep = queue(BAD, FINE)
+    torch.cuda.synchronize()
+    got = m.step(video, audio, 0.7, 0.4)
+    m.synchronize()
+    m.close()
+    assert all(np.array_equal(g, w) for g, w in zip(got, want))
+    assert H.lib().h3k_wait_selftest(1_000_000, stream()) == H.H3_ERR_DEVICE  # a failure of its own, reported and cleared
+    assert H.lib().h3k_check(ctypes.c_void_p(stream())) == H.H3_ERR_DEVICE
+    assert "starts" in H.lib().h3_last_error().decode()
+    sync()
+    del keep
+
+
+@pytest.mark.gpu
+def test_each_caller_has_a_status_word_of_its_own(cuda):
+    """Two callers on two streams, one with bad starts: its word says so, the other's and h3k_check do not. A word is written by every run."""
+    words = torch.full((4,), -1, dtype=torch.int32, device=cuda)
+    keep = []
+    torch.cuda.synchronize()
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    for side, word, q_start in ((sides[0], words[0:1], BAD), (sides[1], words[1:2], FINE)):
+        with torch.cuda.stream(side):
+            keep.append(queue(q_start, FINE, word))
+    torch.cuda.synchronize()
+    assert words.tolist() == [1, 0, -1, -1]
+    sync()
+    keep.append(queue(FINE, [0, 10, 15, 21], words[0:1]))
+    keep.append(queue([0] * 40 + [20], [0] * 41, words[2:3]))
+    keep.append(queue([0], [0], words[3:4]))  # no document: nothing to find
+    torch.cuda.synchronize()
+    assert words.tolist() == [1, 0, 0, 0]
+    sync()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [20, 700])
+def test_a_status_word_follows_the_starts_of_a_replayed_graph(cuda, rows):
+    word = torch.zeros(1, dtype=torch.int32, device=cuda)
+    at = torch.tensor([0, 3, 9, rows], dtype=torch.int32, device=cuda)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        keep = queue(at, at, word, rows)
+    for starts_now, want in (([0, 3, 9, rows], 0), ([0, 9, 3, rows], 1), ([0, 3, 9, rows + 1], 1), ([0, 0, 0, 0], 0)):
+        at.copy_(torch.tensor(starts_now, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert word.item() == want
+    sync()
+    del keep
