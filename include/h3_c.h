@@ -435,7 +435,7 @@ typedef struct h3k_packed_args {
     int32_t type;                                     /* H3K_BF16 or H3K_F16 */
     int32_t heads, kv_heads, head_dim;                /* heads a multiple (1 to 64) of kv_heads; head_dim 64 or 128 */
     int32_t q_rows, k_rows;                           /* rows of q and out, of k and v */
-    int32_t docs, prefix;
+    int32_t docs, prefix;                             /* at most 2^30 documents */
     const int32_t* q_start; /* [docs + 1], ascending, in device memory, read when the work runs (a replayed graph sees */
     const int32_t* k_start; /* new values): after starts out of order or out of the rows, which `status` or h3k_check tells, */
                             /* what the call wrote is not to be used; nothing outside the rows is touched */

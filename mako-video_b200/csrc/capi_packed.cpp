@@ -51,6 +51,7 @@ h3::Fp4 to_format(const char* call, int32_t format)
     return h3::Fp4(format);
 }
 
+constexpr int32_t kMostDocs = 1 << 30;    // the device's steps past the last one's start are still ints
 constexpr int32_t kMostRows = 0x7fffff80; // in whole scale tiles of 128 rows, still an int
 
 void check_rows(const char* call, int32_t rows, int32_t K)
@@ -177,6 +178,7 @@ int h3k_attention_packed(const h3k_packed_args* a, void* stream)
         need(a->heads > 0 && a->kv_heads > 0 && a->heads % a->kv_heads == 0 && a->heads / a->kv_heads <= 64 && a->kv_heads <= 65535, call,
              "heads must be a multiple (at most 64) of kv_heads");
         need(a->q_rows >= 0 && a->k_rows >= 0 && a->docs >= 0, call, "a negative number of rows or documents");
+        need(a->docs <= kMostDocs, call, "more than 2^30 documents");
         need(a->prefix >= 0 && a->prefix <= a->k_rows, call, "the prefix must lie in the key rows");
         need(a->scale >= 0.f && std::isfinite(a->scale), call, "the scale must be positive (0: 1 / sqrt(head_dim))");
         need(aligned(a->status, 4), call, "a pointer is not aligned");

@@ -463,3 +463,10 @@ def test_a_status_word_follows_the_starts_of_a_replayed_graph(cuda, rows):
         assert word.item() == want
     sync()
     del keep
+
+
+@pytest.mark.parametrize("docs", [2 ** 30 + 1, 2 ** 31 - 33, 2 ** 31 - 1])
+def test_refuses_more_documents_than_the_lookup_can_number(docs):
+    a = H.h3k_packed_args(**(GOOD | dict(q_rows=1, kv_heads=4, docs=docs)))
+    assert H.lib().h3k_attention_packed(ctypes.byref(a), None) == H.H3_ERR_ARG
+    assert "documents" in H.lib().h3_last_error().decode()
