@@ -391,7 +391,8 @@ int h3k_layer_norm(const float* x, int32_t rows, int32_t d, const float* w, cons
  *   row_scale  fp32 [rows], H3K_FP4_NV only
  * H3K_FP4_MX: blocks of 32, scale 2^e as byte e + 127 (255: NaN). H3K_FP4_NV: blocks of 16, e4m3 scales.
  * All pointers are device memory of the current device, 16-byte aligned (row_scale 4), an output's apart from the others';
- * work is queued on `stream`, and the calls may be captured into a graph. At most 2^31 - 128 rows; 0: nothing is done. */
+ * work is queued on `stream`, and the calls may be captured into a graph. At most 2^31 - 128 rows
+ * (0: nothing is done) of at most 2^31 - 256 values; a product has at most 2^31 - 256 rows and columns. */
 #define H3K_FP4_MX 0
 #define H3K_FP4_NV 1
 #define H3K_BF16 0 /* element types */

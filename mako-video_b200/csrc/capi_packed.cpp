@@ -53,12 +53,13 @@ h3::Fp4 to_format(const char* call, int32_t format)
 
 constexpr int32_t kMostDocs = 1 << 30;    // the device's steps past the last one's start are still ints
 constexpr int32_t kMostRows = 0x7fffff80; // in whole scale tiles of 128 rows, still an int
+constexpr int32_t kMostK = 0x7fffff00;    // in whole stages of 256 values, and a product's rows and columns in whole tiles of 256
 
 void check_rows(const char* call, int32_t rows, int32_t K)
 {
     need(rows >= 0, call, "a negative number of rows");
     need(rows <= kMostRows, call, "more than 2^31 - 128 rows");
-    need(K > 0 && K % 32 == 0, call, "K must be a positive multiple of 32");
+    need(K > 0 && K % 32 == 0 && K <= kMostK, call, "K must be a positive multiple of 32, at most 2^31 - 256");
 }
 
 } // namespace
@@ -125,7 +126,7 @@ int h3k_gemm_fp4(const void* A, const void* A_scales, const void* B, const void*
         need(a, call, "null argument");
         check_rows(call, a->M, a->K);
         need(a->N > 0 && a->N % 8 == 0, call, "N must be a positive multiple of 8");
-        need(a->N <= kMostRows, call, "more than 2^31 - 128 columns");
+        need(a->M <= kMostK && a->N <= kMostK, call, "more than 2^31 - 256 rows or columns");
         need(epilogue >= H3K_EPI_BF16 && epilogue <= H3K_EPI_SWIGLU, call, "unknown epilogue");
         need(a->a_chunks <= 1 && a->a_rows_stride == 0 && (a->lda == 0 || a->lda == a->K) && (a->ldb == 0 || a->ldb == a->K), call,
              "packed rows are contiguous: no chunks or pitches");

@@ -478,7 +478,7 @@ void quant(const void* x, int64_t ldx, int rows, int K, void* codes, void* scale
     auto* sc = static_cast<uint8_t*>(scales);
     const int warps = (runs + 32 * QUANT_RUNS - 1) / (32 * QUANT_RUNS);
     if constexpr (F == Fp4::nv && T != Elem::f32) {
-        const int threads = 32 * warps, held = num_sms() * std::max(1, std::min(2048 / threads, 220000 / (RING * K * 2 + 1200)));
+        const int threads = 32 * warps, held = num_sms() * std::max(1, int(std::min<int64_t>(2048 / threads, 220000 / (int64_t(RING) * K * 2 + 1200))));
         // four rows a CTA at least, and then more CTAs: 4128 x 13824 takes 32 us by two CTAs a place and 37 by four, 4128 x 2048, of
         // one row a CTA, 8.4 against 6.8 by the other kernel
         if (warps > 1 && threads <= QUANT_THREADS && all_rows >= 4 * held) {

@@ -564,3 +564,17 @@ def test_pairs_that_follow_one_another_at_once(cuda, f):
     sync()
     for w, (A, B, out, args) in zip(want, calls):
         assert torch.equal(out[0], w) and torch.equal(out[1], w)
+
+
+def test_sizes_whose_whole_tiles_leave_an_int_are_refused():
+    """K, and a product's rows and columns, are rounded up to whole steps of up to 256."""
+    L, most = H.lib(), 0x7fffff00
+    assert H.fp4_sizes(1, most, F4.NV) == (most // 2, most // 64 * 512)
+    for K in (most + 32, 0x7fffffe0):
+        for f in FORMATS:
+            refused(L.h3k_fp4_sizes(1, K, f, None, None), "K must be")
+        refused(L.h3k_quant_rows_fp4(BASE, H.BF16, 0, 1, K, F4.MX, BASE, BASE, None, None), "K must be")
+        refused(L.h3k_dequant_rows_fp4(BASE, BASE, None, 1, K, F4.MX, H.BF16, BASE, K, None), "K must be")
+    for change, text in ((dict(M=most + 1), "rows"), (dict(N=most + 8), "columns"), (dict(K=most + 32), "K must be")):
+        a = H.h3k_gemm_args(**(dict(M=1, N=256, K=64, out=BASE, ldo=0x7fffffff // 8 * 8) | change))
+        refused(L.h3k_gemm_fp4(BASE, BASE, BASE, BASE, F4.MX, ctypes.byref(a), H.EPI_BF16, None), text)
