@@ -229,8 +229,15 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr, uint32_t rank)
     return v;
 }
 
-// g / (1 + e^-g); the quotient within 2 ulp (0 once e^-g is above 2^126, where it is below 2^-119)
-__device__ __forceinline__ float silu_approx(float g) { return __fdividef(g, 1.0f + __expf(-g)); }
+// silu: g / (1 + e^-g), by the approximate reciprocal (1 ulp), which the rounding to bf16 hides. Both sides are a sixteenth, since the
+// reciprocal of a number above 2^126 would be flushed to 0: the result is 0 only where e^-g / 16 is (g below -90.1,
+// where silu is below 2^-123). As a division in full precision, 512 x 27648 x 5120 takes 57 us instead of 33.
+__device__ __forceinline__ float silu_approx(float g)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(0.0625f + ex2_approx(fmaf(g, -1.4426950408889634f, -4.0f))));
+    return g * 0.0625f * r;
+}
 
 // First column, within the tile, of the chunk c (of four of 32 columns) that an epilogue thread of a half holds: the SwiGLU
 // pairs gate column j with value column 128 + j, so a thread takes 64 of both; else 128 columns in a row.

@@ -578,3 +578,22 @@ def test_sizes_whose_whole_tiles_leave_an_int_are_refused():
     for change, text in ((dict(M=most + 1), "rows"), (dict(N=most + 8), "columns"), (dict(K=most + 32), "K must be")):
         a = H.h3k_gemm_args(**(dict(M=1, N=256, K=64, out=BASE, ldo=0x7fffffff // 8 * 8) | change))
         refused(L.h3k_gemm_fp4(BASE, BASE, BASE, BASE, F4.MX, ctypes.byref(a), H.EPI_BF16, None), text)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K", [(3, 64), (3, 576), (300, 64)], ids=["one stage", "split", "pairs"])
+def test_swiglu_of_gates_far_below_zero(cuda, M, K):
+    """Gates from -80 to -88.5, whose sigmoids are down to 2^-127.7, with values that make up for them: bias alone sets both, the
+    product is 0."""
+    F = 128
+    codes = lambda n: torch.zeros(n, K // 2, dtype=torch.uint8, device=cuda)
+    tiles = lambda n: torch.zeros(H.fp4_sizes(n, K, F4.MX)[1], dtype=torch.uint8, device=cuda)
+    gate, up = torch.linspace(-80, -88.5, F, device=cuda), torch.exp2(torch.linspace(100, 126, F, device=cuda))
+    bias = torch.cat([gate, up])
+    out = torch.zeros(M, F, device=cuda, dtype=torch.bfloat16)
+    product((codes(M), tiles(M), None), (codes(2 * F), tiles(2 * F), None), F4.MX, H.EPI_SWIGLU, out=out, ldo=F, bias=bias)
+    g = gate.double()
+    want = g * sigmoid(g) * up.double()
+    # fp32: the exponential of a number near 88 is off by its argument's rounding in base 2 (128 x 2^-24) and 2 ulp; sum, quotient (2 ulp)
+    # and products by 2^-21 in all; then one rounding to bf16
+    assert ((out - want).abs() <= (2.0 ** -8 + 2.0 ** -15) * want.abs()).all(), ((out - want).abs() / want.abs()).max()
