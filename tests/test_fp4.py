@@ -597,3 +597,70 @@ def test_swiglu_of_gates_far_below_zero(cuda, M, K):
     # fp32: the exponential of a number near 88 is off by its argument's rounding in base 2 (128 x 2^-24) and 2 ulp; sum, quotient (2 ulp)
     # and products by 2^-21 in all; then one rounding to bf16
     assert ((out - want).abs() <= (2.0 ** -8 + 2.0 ** -15) * want.abs()).all(), ((out - want).abs() / want.abs()).max()
+
+
+def check_exactly(x, cuda):
+    """NV codes, scales and row scales of fp32 rows, bit for bit, ties included."""
+    got_codes, got_tiles, row = gpu_quantise(x.to(cuda), F4.NV)
+    codes, bytes_, want_row, _ = F4.quantise(x.double().numpy(), F4.NV)
+    packed, tiles = F4.pack(codes, bytes_)
+    np.testing.assert_array_equal(got_tiles.cpu().numpy(), tiles)
+    np.testing.assert_array_equal(row.cpu().numpy().astype(np.float64), want_row)
+    got, _ = F4.unpack(got_codes.cpu().numpy().reshape(x.shape[0], -1), tiles, F4.NV)
+    np.testing.assert_array_equal(np.where(got == 8, 0, got), codes)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("power", [-126, -120, -118, -107, -30, 0, 100, 116])
+def test_quantise_fp32_on_and_beside_every_border_of_every_scale(cuda, power):
+    """As above for fp32, up to four steps to either side. (x has 24 bits and t c at most seven, so an x beside the border is
+    more than half a step of the quotient from it: one correct rounding does not reach it.)"""
+    scales = [c for c in F4.e4m3_values().tolist() if 0 < c <= 320]
+    borders = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
+    blocks = [np.concatenate([[6 * c], borders * c, -borders * c, [0.0]]) for c in scales]
+    x = np.concatenate([[2047.0] + [1.0] * 15] + blocks + [np.zeros(16)] * ((len(blocks) + 1) % 2))
+    x = torch.from_numpy(np.stack([x] * 9) * 2.0 ** power).float()
+    bits = x.view(torch.int32)
+    inner = torch.ones(x.shape[1], dtype=torch.bool)
+    inner[::16] = False
+    inner &= x[0] != 0
+    for i, steps in enumerate((0, 1, -1, 2, -2, 3, -3, 4, -4)):
+        bits[i, inner] += steps
+    check_exactly(x, cuda)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["normal", "ties", "wide"])
+@pytest.mark.parametrize("rows,K", [(1, 32), (130, 160), (33, 2048), (5, 4160), (7, 8224), (3, 40000)])
+def test_quantise_fp32_exactly(cuda, kind, rows, K):
+    check_exactly(torch.from_numpy(rows_like(rows, K, rows + K + 1, kind)).clamp(-3e38, 3e38).float(), cuda)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f", FORMATS)
+@pytest.mark.parametrize("M,heads,per,K,spare", [(300, 8, 1, 96, 5), (129, 8, 4, 512, 0), (1, 16, 2, 64, 2), (100, 52, 52, 96, 0), (100, 52, 13, 96, 3), (128, 56, 7, 288, 1)])
+def test_product_qkv_for_several_ranks(cuda, f, M, heads, per, K, spare):
+    """Heads in groups of `per`, each with a block of its own behind the one before; pairs of CTAs, and at most 128 rows by many single
+    ones. Rows behind M of every block stay as they are."""
+    inner, ranks = heads * 128, heads // per
+    A, B = operand(M, K, f, M, cuda), operand(3 * inner, K, f, K, cuda, 0.1)
+    bias = torch.randn(3 * inner, device=cuda) * 0.1
+    wq, wk = (1 + 0.1 * torch.randn(128, device=cuda) for _ in range(2))
+    angle = torch.rand(M, 48, device=cuda, dtype=torch.float64) * 6.28
+    rope = torch.stack([angle.cos(), angle.sin()], 2).float().contiguous()
+    out = torch.full((ranks + 1, M + spare, 3, per, 128), 7.0, device=cuda, dtype=torch.bfloat16)
+    product(A, B, f, H.EPI_QKV, out=out, bias=bias, rope=rope, qn_w=wq, kn_w=wk, inner=inner, heads_per_rank=per, rows_local=M + spare)
+    y = (A[3] @ B[3].T + bias.double()).view(M, 3, heads, 128)
+    t = (bound(A, B) + 2.0 ** -22 * (A[3] @ B[3].T + bias.double()).abs()).view(M, 3, heads, 128)
+    want, tol = y.clone(), t.clone()
+    c, s = rope[:, None, :, 0].double(), rope[:, None, :, 1].double()
+    for sec, w in ((0, wq), (1, wk)):
+        rms = (y[:, sec].square().mean(-1, keepdim=True) + 1e-6).sqrt()
+        v = y[:, sec] / rms * w.double()
+        want[:, sec, :, :48], want[:, sec, :, 48:96], want[:, sec, :, 96:] = v[..., :48] * c - v[..., 48:96] * s, v[..., 48:96] * c + v[..., :48] * s, v[..., 96:]
+        e = t[:, sec] / rms * w.abs().double()
+        tol[:, sec] = 2 * (2 * e.amax(-1, keepdim=True) * (1 + v.abs()) + 2.0 ** -20 * v.abs().amax(-1, keepdim=True))  # as in test_product_qkv
+    tol = tol + 2.0 ** -8 * want.abs()
+    got = out[:ranks, :M].permute(1, 2, 0, 3, 4).reshape(M, 3, heads, 128)  # [rank][row][3][slot] -> [row][3][head]
+    assert ((got - want).abs() <= tol).all()
+    assert (out[:ranks, M:] == 7).all() and (out[ranks] == 7).all()
