@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(FEW_NT, 2) small_runs_kernel(const __grid_cons
                 uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + size_t(row) * p.out_stride + head * HD) + quad;
 #pragma unroll
                 for (int i = 0; i < HD / 8; ++i)
-                    dst[i * 4] = pack2<F16>(o[i][2 * r] * inv, o[i][2 * r + 1] * inv);
+                    dst[i * 4] = l[r] == 0.f ? 0u : pack2<F16>(o[i][2 * r] * inv, o[i][2 * r + 1] * inv); // (0 times a value may be a NaN)
             }
         return;
     }
@@ -861,11 +861,11 @@ __device__ __forceinline__ void attend(const PkMaps& maps, const PkArgs& p, cons
                 if (n > 0) {
                     tmem_ld32(tO + c * 32, o);
                     tmem_wait_ld();
-                } else {
+                }
+                if (l == 0.f) // O may hold 0 times an infinity or a NaN
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
                         o[i] = 0;
-                }
                 if (valid) {
                     uint4* d4 = reinterpret_cast<uint4*>(dst + c * 32);
 #pragma unroll

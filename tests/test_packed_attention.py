@@ -470,3 +470,24 @@ def test_refuses_more_documents_than_the_lookup_can_number(docs):
     a = H.h3k_packed_args(**(GOOD | dict(q_rows=1, kv_heads=4, docs=docs)))
     assert H.lib().h3k_attention_packed(ctypes.byref(a), None) == H.H3_ERR_ARG
     assert "documents" in H.lib().h3_last_error().decode()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type", list(TYPES))
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("docs,rows,keys", [(1, 1, 40), (1, 1, 9000), (40, 30, 60), (3, 300, 200), (3, 40, 5000), (2, 600, 2000)])
+def test_rows_whose_scores_are_all_minus_infinity_are_zeros_whatever_the_values(cuda, type, dim, docs, rows, keys):
+    """The even documents' keys are -infinity and their values infinities and NaNs; the odd ones' rows are as ever."""
+    q_start, k_start = starts([rows] * docs), starts([keys] * docs)
+    g = torch.Generator(device=cuda).manual_seed(rows)
+    q, k, v = (torch.randn(n, 2, dim, generator=g, device=cuda).to(TYPES[type][0]) for n in (docs * rows, docs * keys, docs * keys))
+    q, out = q.abs() + 0.1, torch.full_like(q, 7.0)
+    for d in range(0, docs, 2):
+        k[k_start[d]:k_start[d + 1]] = float("-inf")
+        v[k_start[d]:k_start[d + 1]:2], v[k_start[d] + 1:k_start[d + 1]:2] = float("inf"), float("nan")
+    at_q, at_k = (torch.tensor(s, dtype=torch.int32, device=cuda) for s in (q_start, k_start))
+    call(q, k, v, out, at_q, at_k, 0)
+    out, q, k, v = (t.view(docs, -1, 2, dim) for t in (out, q, k, v))
+    assert (out[0::2] == 0).all()
+    for d in range(1, min(docs, 4), 2):
+        compare(out[d], *expected(q[d], k[d], v[d], [0, rows], [0, keys], 0, dim ** -0.5, out[d]))
