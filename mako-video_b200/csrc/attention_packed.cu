@@ -36,9 +36,9 @@ constexpr float kRescaleThreshold = 8.0f;  // log2 units
 // one is a third V slot.
 constexpr int KST = 3, VST = 2;
 constexpr int NT = 64 + 256;
-// 128-key blocks of a CTA's before more of its cluster join in, and of theirs at least: a block takes 2.3 us, writing, joining and
-// storing the parts of 256 rows about 8 (600 rows and keys of 10 heads in 16.3 us by one CTA, 19.3 by two; 3000 keys in 24.5 by
-// six, 30.2 by three).
+// 128-key blocks of a CTA's before more of its cluster join in, and of theirs at least: a block of two query tiles takes 1.9 us, writing,
+// joining and storing the parts of 256 rows about 8 (256 rows of 10 heads of 128 on 1000 keys in 22.2 us by one CTA, 21.4 by two; on
+// 3000 keys in 50.7 by one, 29.3 by three, 24.3 by six).
 constexpr int LEAST = 4;
 constexpr int MAX_SPLIT = 8; // CTAs of a cluster
 
@@ -141,7 +141,10 @@ __device__ __forceinline__ Document find_document(const PkArgs& p, int slot, int
         uint32_t yes;
         int tile;
         if (p.docs <= 32) {
-            // longest first: a document's slots follow those of all with more keys (of as many: with lower numbers)
+            // Longest first: a document's slots follow those of all with more keys (of as many: with lower numbers). 32 clips of 100 to
+            // 1270 rows and 6 heads of 128 take 74 us so and 82 by row number, 32 of 100 rows and 6 heads of 64 12.5 and 14, 5
+            // documents of 33024 rows 590 and 600; 32 of 60 rows and 20 heads 28 and 26.5. For more documents than lanes the
+            // order would take as many steps for each document as there are.
             const bool rows = in && q0 >= 0 && q1 > q0 && q1 <= p.q_rows;
             const int runs = rows ? (q1 - q0 - 1) / run + 1 : 0, keys = max(k1, p.prefix) - max(k0, p.prefix);
             int before = 0;
@@ -230,8 +233,8 @@ __device__ __forceinline__ uint32_t parts_of(int blocks, int least, uint32_t mos
 //            would be nearly empty and, at 1400 clocks for 128 keys, slower than HBM. The warps have the same rows and take
 //            16 keys of each block; their parts, and then the cluster's, are joined in a fixed order.
 //   by rows  short documents: 64 / group query rows a run, the warps' rows are different ones. A CTA is a fraction of the big
-//            kernel's, starts faster, and two fit an SM: 24 documents of 64 rows and keys and 6 heads of 64 take 5.5 us against
-//            9.1 and 13.5 by keys, of 128 dims 7.0 against 10.2 and 16.4.
+//            kernel's, starts faster, and two fit an SM: 24 documents of 64 rows and keys and 6 heads of 64 take 5.2 us against
+//            8.3 and 13.2 by keys, of 128 dims 6.6 against 9.3 and 15.8.
 // S (16 x 16 keys) = Q K^T: Q's fragments in registers, K's by ldmatrix; P stays in registers (an MMA's sums are the next
 // one's A fragment); O (16 x HD) += P V, V's fragments by ldmatrix.trans. Keys past a block's end get -infinity and V 0.
 constexpr int FEW_ROWS = 16, FEW_KEYS = 64, FEW_STAGES = 3, FEW_WARPS = 4, FEW_NT = 32 + 32 * FEW_WARPS, FEW_SPLIT = 16;
@@ -1033,11 +1036,13 @@ void launch(const PackedAttnParams& p, const PkMaps& maps, const PkArgs& a, cuda
     // (the longest: UNEVEN times as many keys). A form takes the waves of its runs, and at least its longest run. The constants
     // are fits to 1343 calls (1 to 200 documents of 1 to 200 rows on 40 to 6000 keys, even and uneven, four to ten kinds of heads,
     // each in every form): the form so chosen takes 2.3% longer than the fastest one, in the mean; a rule on rows alone 15%, at
-    // worst 91 us for 12.8 (heads of 64, 8 rows of 8 shared heads on 6000 keys).
+    // worst 91 us for 12.8 (heads of 64, 8 rows of 8 shared heads on 6000 keys). What they know nothing of is one document far longer than
+    // the others, which is hardly split: 16 documents of a row, 8 heads, 15 on 40 keys and one on 30000 take 118 us (37 by
+    // clusters of eight), 200 of 8 rows of 8 shared heads, 199 on 100 keys and one on 20000, 488 (67 by tiles in clusters of five).
     constexpr double UNEVEN = 1.6;
     constexpr double KEYS_ALONE = HD == 128 ? 0.55 : 0.38, KEYS_FULL = HD == 128 ? 0.7 : 0.55; // 64 keys of a run: alone, in a full device
     constexpr double ROWS_BLOCK = HD == 128 ? 2.4 : 1.3;                                       // 64 keys
-    constexpr double TILES_BLOCK = HD == 128 ? 1.1 : 0.9;                                      // 128 keys
+    constexpr double TILES_BLOCK = HD == 128 ? 1.1 : 0.9;                                      // 128 keys of the mean run
     const double docs = p.docs, keys = p.prefix + (p.k_rows - p.prefix) / docs, stacked = std::ceil(double(p.q_rows) * a.group / docs);
     auto runs_of = [&](Kernel k) { return docs * p.kv_heads * std::ceil(stacked / (run_rows[k] * a.group)); };
     const double blocks64 = std::ceil(keys / 64), long64 = std::ceil(blocks64 * (p.docs > 1 ? UNEVEN : 1));

@@ -188,7 +188,7 @@ __device__ __forceinline__ uint2 encode(const Run<T>& x, uint32_t most, float rg
             // x / c has to be exact where it lies on the border t of two codes, where ties go by the code, and on its side of it
             // elsewhere. x = t c: the reciprocal of an e4m3 number rounded to nearest is 1 / c (1 + d) with 0 <= d < 2^-24 (so
             // for all eight significands), and t (1 + d) rounded towards zero is t. Else x / c is 2^-13 or more from t (x has 11 bits at
-            // most, t c seven), far more than d and the rounding. (33024 x 13824 in 196 us so, 230 by the residual.)
+            // most, t c seven), far more than d and the rounding. (33024 x 13824 in 205 us so, 230 by the residual.)
             float k = inv * rg;
             if (rg > 0x1p118f) { // rows below 2^-107: k could overflow
                 k = inv;
@@ -328,8 +328,9 @@ __global__ void __launch_bounds__(QUANT_THREADS, 2) quant_fp4_kernel(const void*
 
 // Many nv rows of 16-bit values: all threads of a row wait for its last value before they go on, and few rows fit an SM's
 // registers. So CTAs walk rows, which bulk copies bring into shared memory one ahead of them, and there are up to four times
-// as many CTAs as an SM holds, at different places in their rows: 33024 x 5120 in 69 us (6.3 TB/s) against 84 by the kernel
-// above, x 2048 in 31 against 33, x 13824 in 200 against 270. (A ring of three rows: 73, 33, 215; as many CTAs as fit: 81 at 5120.)
+// as many CTAs as an SM's threads and shared memory hold (registers hold fewer: 8 of the 10 counted at K = 5120), at different
+// places in their rows: 33024 x 5120 in 67 to 70 us (6.3 TB/s) against 84 by the kernel above, x 2048 in 31 against 33, x 13824
+// in 205 against 270. (A ring of three rows: 73, 33, 215; as many CTAs as fit: 81 at 5120.)
 constexpr int RING = 2; // rows
 template <Elem T>
 __global__ void __launch_bounds__(QUANT_THREADS, 2) quant_many_rows_kernel(const void* x, int64_t ldx, int rows, int K, uint8_t* codes, uint8_t* scales,
@@ -381,8 +382,8 @@ __global__ void __launch_bounds__(QUANT_THREADS, 2) quant_many_rows_kernel(const
         }
         // A wait that gave up, of whichever thread, ends the CTA: all of it, so that no warp waits at the barrier for one that has
         // left, and not before its copies have landed. (Another kernel's failure ends waits long before their time, so that
-        // nothing else says that they have.) It goes with the maxima, as what no magnitude is: a
-        // barrier that votes costs 2 to 5% of the call.
+        // nothing else says that they have.) It goes with the maxima, as what no magnitude is: a barrier that votes costs 2 to
+        // 5% of the call.
         constexpr uint32_t LATE = 0xffffffffu;
         all = __reduce_max_sync(0xffffffffu, late ? LATE : all);
         if (lane_id() == 0)

@@ -11,12 +11,12 @@
 // Three forms:
 //   pair   (more than 128 rows, or few tiles) the two CTAs of a cluster share a tile of 256 x 256: each loads its 128 rows of A and half of
 //          B's, the first CTA issues for both (cta_group::2). A stage is 38 KB instead of 54 and five fit: at 54 KB in 512
-//          clocks an SM's share of the L2 bandwidth, not the tensor core, sets the pace. 33024 x 15360 x 5120 takes 0.97 ms
-//          (5.4 PFLOP/s; tensor pipe 77% at the 1.45 GHz that the power limit leaves) against 1.19 in single CTAs, about
+//          clocks an SM's share of the L2 bandwidth, not the tensor core, sets the pace. 33024 x 15360 x 5120 takes 1.03 ms
+//          (5.0 PFLOP/s; tensor pipe 77% at the 1.45 GHz that the power limit leaves) against 1.26 in single CTAs, about
 //          0.13 of it the output's stores. The second CTA's loads complete on the first one's barriers; its thread
 //          telling the first by a remote arrival a stage took 1.5 ms.
 //   tiles  (at most 128 rows, more tiles of 128 x 256 than half the SMs) a CTA walks such tiles: 1 row of 27648 columns and
-//          K = 5120 in 22.8 us against 28.8 by pairs, whose second CTA would have no rows
+//          K = 5120 in 21.6 us against 28.0 by pairs, whose second CTA would have no rows
 //   split  (fewer such tiles, of few rows or long K: the rule is in launch()) the K of a tile is split over the CTAs of a
 //          cluster; they leave their sums in shared memory and each finishes a share of the tile from all of them, in order
 //
@@ -726,8 +726,8 @@ bool launch(const void* A, const void* a_scales, const void* B, const void* b_sc
                 break;
         // Against pairs of 128 columns a CTA, with which a stage takes 0.31 us instead of 0.6 (its share of B is half, the ring
         // deeper): the parts' sums take 4 us through the cluster's shared memory for 128 rows and nearly none for one. K = 5120:
-        // 1 row of 5120 columns takes 9.1 us by seven parts and 12.5 by pairs, 64 rows 11.1 and 12.6, 128 rows 13.3 and 13.0;
-        // 128 rows of 15360 columns 18.4 by two parts and 14.9 by pairs.
+        // 1 row of 5120 columns takes 7.8 us by seven parts and 11.0 by pairs, 64 rows 8.9 and 11.4, 128 rows 11.0 and 11.7;
+        // 128 rows of 15360 columns 18.4 by two parts and 14.8 by pairs, 300 rows of 5120 15.3 by parts and 12.8 by pairs.
         const long long stages = (p.K + KSTAGE - 1) / KSTAGE;
         if (split < 2 || stages * (split - 2) * 8 <= (long long)(std::min(p.M, BM) - 32) * split)
             return false;
