@@ -664,3 +664,24 @@ def test_product_qkv_for_several_ranks(cuda, f, M, heads, per, K, spare):
     got = out[:ranks, :M].permute(1, 2, 0, 3, 4).reshape(M, 3, heads, 128)  # [rank][row][3][slot] -> [row][3][head]
     assert ((got - want).abs() <= tol).all()
     assert (out[:ranks, M:] == 7).all() and (out[ranks] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f", FORMATS)
+@pytest.mark.parametrize("K", [64, 1056], ids=["pair", "split"])
+@pytest.mark.parametrize("N", [8, 264, 512])
+def test_one_row_of_any_pitch_in_every_epilogue(cuda, f, K, N):
+    """A single row has no pitch to check: ldo and ldx of 3."""
+    A, B = operand(1, K, f, 1, cuda), operand(N, K, f, 2, cuda, 0.1)
+    y = A[3] @ B[3].T
+    t = bound(A, B) + 2.0 ** -22 * y.abs()
+    for epi, dtype in ((H.EPI_F32, torch.float32), (H.EPI_BF16, torch.bfloat16)):
+        out = torch.full((N + 8,), 7.0, device=cuda, dtype=dtype)
+        product(A, B, f, epi, out=out, ldo=3)
+        assert ((out[:N] - y[0]).abs() <= (t + (2.0 ** -8 * y.abs() if dtype == torch.bfloat16 else 0))[0]).all() and (out[N:] == 7).all()
+    x, mod = torch.randn(N + 8, device=cuda), torch.randn(1, 6, N, device=cuda)
+    before, idx = x.clone(), torch.zeros(1, dtype=torch.uint8, device=cuda)
+    product(A, B, f, H.EPI_GATE_RESID, x=x, ldx=3, mod=mod, mod_idx=idx, gate_slot=1, dim=N)
+    gate = mod[0, 1].double()
+    want = before[:N].double() + gate * y[0]
+    assert ((x[:N] - want).abs() <= gate.abs() * t[0] + 2.0 ** -23 * (want.abs() + (gate * y[0]).abs())).all() and torch.equal(x[N:], before[N:])
